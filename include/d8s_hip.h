@@ -459,6 +459,135 @@ int d8s_head(const D8sHeadArgs* a, void* stream);
 #define D8S_HEAD_SCRATCH_BYTES (32u << 20)
 int d8s_head_noalloc(const D8sHeadArgs* a, void* stream);
 
+/* ---- A context layer over all the tokens of a study, and its training ----------------------------
+ *
+ * The reference's context layer attends over at most 128 window features (src/knee/models/baseline.py:
+ * 954-977) and its head is trained in torch.  These entry points are the operators of a layer over every
+ * position of the encoder's last map (6144 tokens in a study of 24 slices at 512 px), with their gradients;
+ * no kernel of the reference corresponds to them.  Element types: */
+#define D8S_F32 0
+#define D8S_BF16 1
+#define D8S_F16 2
+
+/* Layer norm over the last dimension: `rows` rows of `width` (1 .. 16384) values of `dtype`, w and b of `wdtype`
+ * (D8S_F32 or dtype).  Rows of x (and dy) are x_stride (dy_stride) elements apart; y and dx are contiguous.
+ *   d8s_layer_norm:           reads x, w, b (0: none); writes y, and mean and rstd [rows] unless both are 0;
+ *   d8s_layer_norm_backward:  reads dy, x, w, mean, rstd; writes dx [rows][width], dw and (unless 0) db [width]
+ *                             of wdtype; `partial` is device memory of d8s_layer_norm_workspace bytes.
+ * Sums are float32 in a fixed order: equal inputs give equal bits. */
+typedef struct D8sNormArgs {
+    const void *x, *w, *b;
+    void* y;
+    float *mean, *rstd;
+    const void* dy;
+    void *dx, *dw, *db;
+    float* partial;
+    uint64_t partial_bytes;
+    int64_t rows, x_stride, dy_stride;
+    int32_t width, dtype, wdtype;
+    float eps;
+} D8sNormArgs;
+
+int d8s_layer_norm(const D8sNormArgs* a, void* stream);
+int d8s_layer_norm_workspace(const D8sNormArgs* a, uint64_t* bytes);
+int d8s_layer_norm_backward(const D8sNormArgs* a, void* stream);
+
+/* Rotary positions of several axes: x and y [B][S][H][D] of dtype with the given strides (elements; the last
+ * dimension is contiguous; y may be x), pos [B][S][axes] (pos_type 0 int32, 1 int64, 2 float32; strides pos_sb,
+ * pos_ss).  The first 2 * pairs channels are turned, the others copied; pair i is channels (i, i + pairs), or
+ * (2 i, 2 i + 1) when `adjacent`.  Pair i turns by pos[axis[i]] * freq[i] whole turns (freq: radians per position
+ * divided by 2 pi); backwards when `inverse`, which is also the gradient. */
+#define D8S_ROTARY_PAIRS 256
+typedef struct D8sRotaryArgs {
+    const void* x;
+    void* y;
+    const void* pos;
+    int64_t x_sb, x_ss, x_sh, y_sb, y_ss, y_sh, pos_sb, pos_ss;
+    int32_t B, S, H, D, pairs, axes, dtype, pos_type, adjacent, inverse;
+    double freq[D8S_ROTARY_PAIRS];
+    uint8_t axis[D8S_ROTARY_PAIRS];
+} D8sRotaryArgs;
+
+int d8s_rotary(const D8sRotaryArgs* a, void* stream);
+
+/* Attention of S tokens within a window and `sinks` first tokens: key j is visible to query i iff j <= i + right,
+ * (j >= i - left or j < sinks) and mask[j] is not 0 (mask 0: all).  A query that sees nothing has zeros, lse -inf
+ * and no gradient; what lies in rows of masked keys is not used.  q, dout [B][S][H][D], k, v [B][S][HK][D] of dtype
+ * (D8S_BF16 or D8S_F16; D 64 or 128; H a multiple of HK, query head h uses key head h / (H / HK)) with the given
+ * strides (elements, the last dimension contiguous); out, dq [B][S][H][D], dk, dv [B][S][HK][D] and lse [B][H][S]
+ * (natural logarithm of the sum of exponentials) contiguous.  Products are of 16 bits with float32 sums; P and dS
+ * are rounded to dtype between two products.  Equal inputs give equal bits.
+ *   d8s_attention:           writes out, and lse unless 0;
+ *   d8s_attention_backward:  reads out and lse beside the inputs; writes dq, dk, dv; `workspace` is device memory of
+ *                            d8s_attention_workspace bytes, 16-byte aligned. */
+typedef struct D8sAttnArgs {
+    const void *q, *k, *v;
+    const uint8_t* mask;       /* [B] rows mask_sb bytes apart */
+    void* out;
+    float* lse;
+    const void* dout;
+    void *dq, *dk, *dv;
+    void* workspace;
+    uint64_t ws_bytes;
+    int64_t q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, do_sb, do_ss, do_sh, mask_sb;
+    int32_t B, S, H, HK, D, dtype, left, right, sinks;
+    float scale;
+} D8sAttnArgs;
+
+int d8s_attention(const D8sAttnArgs* a, void* stream);
+int d8s_attention_workspace(const D8sAttnArgs* a, uint64_t* bytes);
+int d8s_attention_backward(const D8sAttnArgs* a, void* stream);
+
+/* One new token a row against a cache: q [B][H][D], k, v [B][S][HK][D] with strides as above; the token is the last
+ * of its row's lengths[b] (0 .. S, on the device; others are cut to that) and sees keys as in d8s_attention with
+ * right 0 and no mask.  Keys from lengths[b] on are not read.  out [B][H][D] contiguous; length 0 gives zeros.
+ * `workspace`: device memory of d8s_attention_token_workspace bytes (may be 0). */
+typedef struct D8sTokenArgs {
+    const void *q, *k, *v;
+    const int32_t* lengths;
+    void* out;
+    void* workspace;
+    uint64_t ws_bytes;
+    int64_t q_sb, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;
+    int32_t B, S, H, HK, D, dtype, left, sinks;
+    float scale;
+    int32_t pad_;
+} D8sTokenArgs;
+
+int d8s_attention_token(const D8sTokenArgs* a, void* stream);
+int d8s_attention_token_workspace(const D8sTokenArgs* a, uint64_t* bytes);
+
+/* One AdamW step over `count` tensors: p of dtype (n elements, contiguous), g of grad_dtype (D8S_F32 or, beside
+ * float32 or equal p, 16 bits), both moments of all tensors in one array each, tensor i's from element `at` on (a
+ * multiple of D8S_ADAMW_BLOCK, rounded up to whole blocks; the rounding's elements stay zeros).
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * with g multiplied by *grad_scale (device memory) unless that is 0.  bits 32: m and v float32.  bits 8: m holds
+ * int8 codes c of value m_scale (c |c|) / 127^2, v uint8 codes c whose square root is v_scale c^2 / 255^2, with one
+ * scale a block of D8S_ADAMW_BLOCK elements.  `tensors` is host memory, read before the call returns; the step's
+ * numbers are arguments, so a recorded graph repeats the same step. */
+#define D8S_ADAMW_BLOCK 256
+typedef struct D8sAdamwTensor {
+    void* p;
+    const void* g;
+    int64_t n, at;
+} D8sAdamwTensor;
+
+typedef struct D8sAdamwArgs {
+    const D8sAdamwTensor* tensors;
+    void *m, *v;
+    float *m_scale, *v_scale;  /* bits 8 */
+    const float* grad_scale;
+    int64_t step;
+    double lr, beta1, beta2, eps, weight_decay;
+    int32_t count, dtype, grad_dtype, bits;
+} D8sAdamwArgs;
+
+int d8s_adamw(const D8sAdamwArgs* a, void* stream);
+/* The n values (a multiple of D8S_ADAMW_BLOCK) that moments of 8 bits stand for. */
+int d8s_adamw_moments(const void* m_code, const void* v_code, const float* m_scale, const float* v_scale, int64_t n,
+                      float* m, float* v, void* stream);
+
 /* Library identification: "d8s-hip <abi> <source hash> gfx950". */
 const char* d8s_version(void);
 

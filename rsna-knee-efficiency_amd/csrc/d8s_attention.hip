@@ -1,0 +1,835 @@
+// gfx950 kernels of attention within a window of neighbouring tokens and a few first tokens that stay visible, for a
+// context layer over all the tokens of a study: forward, backward, and one new token against a cache; the C ABI is in
+// include/d8s_hip.h.
+//
+// Key j is visible to query i iff j <= i + right, (j >= i - left or j < sinks) and mask[j].  With s = scale q k,
+//   P = softmax over the visible keys (nothing visible: zeros),  o = P v,  lse = log sum exp s (-inf);
+//   dv = P^T do,  dP = do v^T,  dS = P (dP - rowsum(do o)),  dq = scale dS k,  dk = scale dS^T q.
+//
+// The products run on v_mfma_f32_32x32x16 (bf16 or f16, float32 sums), arranged so that what comes out of one product
+// goes into the next from the registers it is in: lane l of a 32 x 32 result holds column l % 32 and the rows
+// r % 4 + 8 (r / 4) + 4 (l / 32) of its 16 registers r, and an operand's lane holds row (or column) l % 32 and eight of
+// the 16 values that are summed over.  Which eight is free as long as both operands agree, so the eight registers
+// 8 s .. 8 s + 7 of a result are an operand as they are, and the other one is read with
+// the same order: rows 16 s + 4 (l / 32) + (0 .. 3) and 8 more, by ds_read_b64_tr_b16, which hands each lane a column
+// of a row-major tile.  So nothing is transposed or exchanged between lanes.
+// Tiles of rows lie in LDS in 16-byte pieces, piece c of row r at c ^ swizzle(r): both ways of reading them (16
+// lanes at one piece of 16 rows; 32 lanes at 4 neighbouring pieces of 4 rows) then touch every bank once.
+#include <hip/hip_runtime.h>
+
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <string>
+
+#include "d8s_elem.h"
+#include "d8s_hip.h"
+#include "d8s_host.h"
+
+namespace {
+
+using namespace d8s;
+
+#define AREQ(cond, msg) \
+    do { if (!(cond)) return d8s_host_fail((int)hipErrorInvalidValue, std::string(what) + ": " + (msg)); } while (0)
+
+constexpr int NT = 256;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <class T>
+using Frag = T __attribute__((ext_vector_type(8)));
+typedef Vec<uint16_t, 8> Raw;                  // 8 elements as they lie in memory
+
+DEV f32x16 mfma(Frag<bf16> a, Frag<bf16> b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+DEV f32x16 mfma(Frag<f16> a, Frag<f16> b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 16-byte pieces of a row of D values, and where piece c of row r lies
+template <int D>
+DEV int piece(int r, int c) {
+    static_assert(D == 64 || D == 128, "row of 8 or 16 pieces");
+    if constexpr (D == 64) {
+        const int k = (r >> 1) & 7;            // rows r and r + 1 fill the banks once: the swizzle goes by pairs
+        return r * 8 + (c ^ ((k & 1) << 2 | (k & 2) | k >> 2));
+    } else {
+        return r * 16 + (c ^ ((r & 3) << 2 | (r >> 2 & 3)));
+    }
+}
+
+// Operand of rows r0 .. r0 + 31, values 16 k .. 16 k + 15 of each
+template <class T, int D>
+DEV Frag<T> rows_frag(const u32x4* tile, int r0, int k, int lane) {
+    const u32x4 v = tile[piece<D>(r0 + lane % 32, 2 * k + lane / 32)];
+    return __builtin_bit_cast(Frag<T>, v);
+}
+
+// Operand of columns d0 .. d0 + 31, summed over the tile's rows r0 .. r0 + 15 in the order of a result's registers
+template <class T, int D>
+DEV Frag<T> cols_frag(const u32x4* tile, int r0, int d0, int lane) {
+    typedef __attribute__((address_space(3))) s16x4* lds;
+    const int i = lane % 16, r = r0 + 4 * (lane / 32) + i / 4;
+    const int c = d0 / 8 + 2 * (lane / 16 & 1) + (i % 4) / 2;
+    const char* lo = (const char*)(tile + piece<D>(r, c)) + 8 * (i & 1);
+    const char* hi = (const char*)(tile + piece<D>(r + 8, c)) + 8 * (i & 1);
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)lo), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)hi);
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    const s16x8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(Frag<T>, v);
+}
+
+template <class T>
+DEV Frag<T> round_frag(const f32x16& x, int s) {
+    Frag<T> f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (T)x[8 * s + j];
+    return f;
+}
+
+DEV int row_of(int r, int lane) { return r % 4 + 8 * (r / 4) + 4 * (lane / 32); }
+
+// Consecutive problems on one XCD's L2: workgroup w runs problem (w % 8) (n / 8) + w / 8 (as far as 8 divides n)
+DEV int xcd_order(int w, int n) {
+    const int per = n / 8;
+    return w < 8 * per ? (w % 8) * per + w / 8 : w;
+}
+
+// The tiles of TILE keys a run of queries i0 .. i1 can see: the first tokens' ones, then the window's
+struct Tiles {
+    int first, start, count;
+    DEV int at(int i) const { return i < first ? i : start + i - first; }
+};
+template <int TILE>
+DEV Tiles tiles_of(const D8sAttnArgs& p, int i0, int i1) {
+    const int lo = max(0, i0 - p.left) / TILE, hi = min((int64_t)p.S - 1, (int64_t)i1 + p.right) / TILE;
+    const int first = min((min(p.sinks, p.S) + TILE - 1) / TILE, lo);
+    return {first, lo, first + hi - lo + 1};
+}
+
+// Whether queries i0 .. i0 + 31 see none, or all, of keys k0 .. k1
+DEV bool none_seen(const D8sAttnArgs& p, int i0, int k0, int k1) {
+    return k0 > (int64_t)i0 + 31 + p.right || (k1 < i0 - p.left && k0 >= p.sinks);
+}
+DEV bool all_seen(const D8sAttnArgs& p, int i0, int k0, int k1) {
+    return k1 <= (int64_t)i0 + p.right && (k0 >= i0 + 31 - p.left || k1 < p.sinks);
+}
+DEV bool seen(const D8sAttnArgs& p, int i, int j) {
+    return j <= (int64_t)i + p.right && (j >= i - p.left || j < p.sinks);
+}
+
+// One thread's share of a tile of ROWS rows, in registers between memory and LDS
+template <int D, int ROWS>
+struct Stage {
+    static constexpr int N = ROWS * D / 8 / NT;
+    Raw v[N];
+    // rows r0 .. of a matrix whose rows are `stride` elements apart; rows past `last` are read as `last`
+    DEV void load(const uint16_t* p, int64_t stride, int r0, int last) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int id = n * NT + threadIdx.x, r = min(r0 + id / (D / 8), last);
+            v[n] = *(const Raw*)(p + r * stride + id % (D / 8) * 8);
+        }
+    }
+    // rows whose bit is not set become zeros (whatever memory holds there)
+    DEV void store(u32x4* tile, uint64_t bits) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int id = n * NT + threadIdx.x, r = id / (D / 8);
+            const u32x4 x = __builtin_bit_cast(u32x4, v[n]);
+            tile[piece<D>(r, id % (D / 8))] = bits >> r & 1 ? x : u32x4{0, 0, 0, 0};
+        }
+    }
+};
+
+// Bit r: key k0 + r exists and is not masked
+DEV uint64_t key_bits(const uint8_t* mask, int S, int k0, int lane) {
+    const int k = k0 + lane;
+    const bool on = k < S && (mask == nullptr || mask[min(k, S - 1)] != 0);
+    return __ballot(on);
+}
+
+// ---- forward --------------------------------------------------------------------------------------
+// A workgroup runs 128 queries of a head, 32 a wave, over the tiles of 64 keys they can see; keys and values go
+// through two LDS buffers, the next tile's loads in flight while one is computed.  A wave forms s transposed (keys x
+// queries), so a query's statistics are one value a lane, and P goes from registers into the second product.
+// The running maximum m is raised, and the sums scaled, only where a tile exceeds it by more than 2^RISE (P stays below
+// 2^RISE, harmless in float32 and in both types), which after a row's first tiles is rare.
+constexpr float RISE = 6.0f;
+
+template <class T, int D>
+__global__ __launch_bounds__(NT, 2) void k_attn(D8sAttnArgs p) {
+    constexpr int TILE = 64, ND = D / 32;
+    __shared__ u32x4 lk[2][TILE * D / 8], lv[2][TILE * D / 8];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int nq = (p.S + 127) / 128, id = xcd_order(blockIdx.x, gridDim.x);
+    const int b = id / (nq * p.H), h = id / nq % p.H, i00 = id % nq * 128, i0 = i00 + 32 * wave;
+    const int hk = h / (p.H / p.HK);
+    const uint16_t* kp = (const uint16_t*)p.k + b * p.k_sb + hk * p.k_sh;
+    const uint16_t* vp = (const uint16_t*)p.v + b * p.v_sb + hk * p.v_sh;
+    const uint8_t* mask = p.mask ? p.mask + b * p.mask_sb : nullptr;
+    const int i = i0 + lane % 32;
+    Frag<T> q[D / 16];
+    {
+        const uint16_t* qp = (const uint16_t*)p.q + b * p.q_sb + h * p.q_sh + (int64_t)min(i, p.S - 1) * p.q_ss;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+            q[k] = __builtin_bit_cast(Frag<T>, *(const Raw*)(qp + 16 * k + 8 * (lane / 32)));
+    }
+    const float c = p.scale * LOG2E;
+    float m = -INFINITY, l = 0.0f;
+    f32x16 acc[ND] = {};
+    const Tiles tiles = tiles_of<TILE>(p, i00, min(i00 + 127, p.S - 1));
+    Stage<D, TILE> sk, sv;
+    int k0 = tiles.at(0) * TILE;
+    uint64_t bits = key_bits(mask, p.S, k0, lane);
+    sk.load(kp, p.k_ss, k0, p.S - 1);
+    sv.load(vp, p.v_ss, k0, p.S - 1);
+    sk.store(lk[0], bits);
+    sv.store(lv[0], bits);
+    __syncthreads();
+    for (int t = 0; t < tiles.count; ++t) {
+        uint64_t next = 0;
+        int k1 = 0;
+        if (t + 1 < tiles.count) {
+            k1 = tiles.at(t + 1) * TILE;
+            next = key_bits(mask, p.S, k1, lane);
+            sk.load(kp, p.k_ss, k1, p.S - 1);
+            sv.load(vp, p.v_ss, k1, p.S - 1);
+        }
+        if (bits != 0 && !none_seen(p, i0, k0, k0 + TILE - 1)) {
+            const u32x4 *tk = lk[t & 1], *tv = lv[t & 1];
+            f32x16 s[2] = {};
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) s[u] = mfma(rows_frag<T, D>(tk, 32 * u, k, lane), q[k], s[u]);
+            if (bits != ~0ull || !all_seen(p, i0, k0, k0 + TILE - 1)) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int j = 32 * u + row_of(r, lane);
+                        s[u][r] = (bits >> j & 1) && seen(p, i, k0 + j) ? s[u][r] : -INFINITY;
+                    }
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+            float t0, t1;
+            swap32(top, t0, t1);
+            top = fmaxf(t0, t1);
+            if (__any(top * c > m * c + RISE)) {
+                const float up = fmaxf(m, top), a = up == -INFINITY ? 1.0f : exp2_((m - up) * c);
+                m = up;
+                l *= a;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[d][r] *= a;
+            }
+            const float mc = m == -INFINITY ? 0.0f : m * c;
+            float sum = 0.0f;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[u][r] = exp2_(__builtin_fmaf(s[u][r], c, -mc));
+                    sum += s[u][r];
+                }
+            l += sum;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const Frag<T> w = round_frag<T>(s[u / 2], u % 2);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) acc[d] = mfma(cols_frag<T, D>(tv, 16 * u, 32 * d, lane), w, acc[d]);
+            }
+        }
+        if (t + 1 < tiles.count) {
+            sk.store(lk[(t + 1) & 1], next);
+            sv.store(lv[(t + 1) & 1], next);
+        }
+        bits = next;
+        k0 = k1;
+        __syncthreads();
+    }
+    float l0, l1;
+    swap32(l, l0, l1);
+    l = l0 + l1;
+    if (i >= p.S) return;
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    if (p.lse && lane < 32) p.lse[((int64_t)b * p.H + h) * p.S + i] = l > 0.0f || l != l ? (m * c + log2f(l)) * LN2 : -INFINITY;
+    T* o = (T*)p.out + (((int64_t)b * p.S + i) * p.H + h) * D + 4 * (lane / 32);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float f[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] = acc[d][4 * g + j] * inv;
+            store_n<T, 4>(o + 32 * d + 8 * g, 4, f);
+        }
+}
+
+// ---- backward: queries ------------------------------------------------------------------------------
+// As the forward pass, with do beside q: P from lse, dP = do v^T transposed, dS, dq += dS k.  It also leaves
+// rowsum(do o) for the keys' kernel.
+DEV float lse2_of(float lse) { return lse == -INFINITY ? INFINITY : lse * LOG2E; }   // (empty row: every P is 0)
+
+template <class T, int D>
+__global__ __launch_bounds__(NT, 2) void k_attn_dq(D8sAttnArgs p, float* delta) {
+    constexpr int TILE = 64, ND = D / 32;
+    __shared__ u32x4 lk[2][TILE * D / 8], lv[2][TILE * D / 8];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int nq = (p.S + 127) / 128, id = xcd_order(blockIdx.x, gridDim.x);
+    const int b = id / (nq * p.H), h = id / nq % p.H, i00 = id % nq * 128, i0 = i00 + 32 * wave;
+    const int hk = h / (p.H / p.HK);
+    const uint16_t* kp = (const uint16_t*)p.k + b * p.k_sb + hk * p.k_sh;
+    const uint16_t* vp = (const uint16_t*)p.v + b * p.v_sb + hk * p.v_sh;
+    const uint8_t* mask = p.mask ? p.mask + b * p.mask_sb : nullptr;
+    const int i = i0 + lane % 32, ic = min(i, p.S - 1);
+    Frag<T> q[D / 16], g[D / 16];
+    float dl = 0.0f;
+    {
+        const int64_t at = 8 * (lane / 32);
+        const uint16_t* qp = (const uint16_t*)p.q + b * p.q_sb + h * p.q_sh + ic * p.q_ss + at;
+        const uint16_t* gp = (const uint16_t*)p.dout + b * p.do_sb + h * p.do_sh + ic * p.do_ss + at;
+        const uint16_t* op = (const uint16_t*)p.out + (((int64_t)b * p.S + ic) * p.H + h) * D + at;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+            q[k] = __builtin_bit_cast(Frag<T>, *(const Raw*)(qp + 16 * k));
+            g[k] = __builtin_bit_cast(Frag<T>, *(const Raw*)(gp + 16 * k));
+            const Frag<T> o = __builtin_bit_cast(Frag<T>, *(const Raw*)(op + 16 * k));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dl = __builtin_fmaf((float)g[k][j], (float)o[j], dl);
+        }
+        float a, c;
+        swap32(dl, a, c);
+        dl = a + c;
+    }
+    const int64_t stat = ((int64_t)b * p.H + h) * p.S + ic;
+    if (lane < 32 && i < p.S) delta[stat] = dl;
+    const float c = p.scale * LOG2E, lse2 = lse2_of(p.lse[stat]);
+    f32x16 acc[ND] = {};
+    const Tiles tiles = tiles_of<TILE>(p, i00, min(i00 + 127, p.S - 1));
+    Stage<D, TILE> sk, sv;
+    int k0 = tiles.at(0) * TILE;
+    uint64_t bits = key_bits(mask, p.S, k0, lane);
+    sk.load(kp, p.k_ss, k0, p.S - 1);
+    sv.load(vp, p.v_ss, k0, p.S - 1);
+    sk.store(lk[0], bits);
+    sv.store(lv[0], bits);
+    __syncthreads();
+    for (int t = 0; t < tiles.count; ++t) {
+        uint64_t next = 0;
+        int k1 = 0;
+        if (t + 1 < tiles.count) {
+            k1 = tiles.at(t + 1) * TILE;
+            next = key_bits(mask, p.S, k1, lane);
+            sk.load(kp, p.k_ss, k1, p.S - 1);
+            sv.load(vp, p.v_ss, k1, p.S - 1);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int ku = k0 + 32 * u;
+            const uint32_t bu = (uint32_t)(bits >> (32 * u));
+            if (bu == 0 || none_seen(p, i0, ku, ku + 31)) continue;
+            const u32x4 *tk = lk[t & 1], *tv = lv[t & 1];
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                s = mfma(rows_frag<T, D>(tk, 32 * u, k, lane), q[k], s);
+                dp = mfma(rows_frag<T, D>(tv, 32 * u, k, lane), g[k], dp);
+            }
+            const bool part = bu != ~0u || !all_seen(p, i0, ku, ku + 31);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = exp2_(__builtin_fmaf(s[r], c, -lse2));
+            if (part) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int j = row_of(r, lane);
+                    s[r] = (bu >> j & 1) && seen(p, i, ku + j) ? s[r] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] *= dp[r] - dl;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const Frag<T> ds = round_frag<T>(s, w);
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+                    acc[d] = mfma(cols_frag<T, D>(tk, 32 * u + 16 * w, 32 * d, lane), ds, acc[d]);
+            }
+        }
+        if (t + 1 < tiles.count) {
+            sk.store(lk[(t + 1) & 1], next);
+            sv.store(lv[(t + 1) & 1], next);
+        }
+        bits = next;
+        k0 = k1;
+        __syncthreads();
+    }
+    if (i >= p.S) return;
+    T* o = (T*)p.dq + (((int64_t)b * p.S + i) * p.H + h) * D + 4 * (lane / 32);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            float f[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] = acc[d][4 * w + j] * p.scale;
+            store_n<T, 4>(o + 32 * d + 8 * w, 4, f);
+        }
+}
+
+// ---- backward: keys and values ----------------------------------------------------------------------
+// A workgroup runs 128 keys of a key head, 32 a wave, over the tiles of 64 queries that see them, one query head of
+// the group after the other, so that dk and dv of shared heads are sums within one workgroup, in a fixed order.  The
+// tiles of the first tokens are seen by every query: their queries are split over `sink_split` workgroups (and all
+// tiles' over `split` where there are fewer tiles than compute units), whose float32 sums k_attn_join adds.
+struct KeySplit {
+    int sink_tiles, sink_split, split;
+};
+
+template <class T, int D>
+__global__ __launch_bounds__(NT, 2) void k_attn_dkv(D8sAttnArgs p, const float* delta, float* part, KeySplit ks) {
+    constexpr int KEYS = 128, TILE = 64, ND = D / 32;
+    __shared__ u32x4 lq[2][TILE * D / 8], lg[2][TILE * D / 8];
+    __shared__ float ls[2][TILE], ld[2][TILE];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int nk = (p.S + KEYS - 1) / KEYS, G = p.H / p.HK;
+    const int items = ks.sink_tiles * ks.sink_split + (nk - ks.sink_tiles) * ks.split;
+    const int id = xcd_order(blockIdx.x, gridDim.x), item = id % items, bh = id / items, b = bh / p.HK, hk = bh % p.HK;
+    const bool sink = item < ks.sink_tiles * ks.sink_split;
+    const int rest = sink ? item : item - ks.sink_tiles * ks.sink_split, n = sink ? ks.sink_split : ks.split;
+    const int kt = (sink ? 0 : ks.sink_tiles) + rest / n, cut = rest % n;
+    const int j0 = kt * KEYS, jw = j0 + 32 * wave, j = jw + lane % 32, jc = min(j, p.S - 1);
+    const uint8_t* mask = p.mask ? p.mask + b * p.mask_sb : nullptr;
+    const bool on = j < p.S && (mask == nullptr || mask[jc] != 0);
+    const uint64_t any = __ballot(on);
+    Frag<T> k[D / 16], v[D / 16];
+    {
+        const uint16_t* kp = (const uint16_t*)p.k + b * p.k_sb + hk * p.k_sh + jc * p.k_ss + 8 * (lane / 32);
+        const uint16_t* vp = (const uint16_t*)p.v + b * p.v_sb + hk * p.v_sh + jc * p.v_ss + 8 * (lane / 32);
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u) {
+            k[u] = __builtin_bit_cast(Frag<T>, *(const Raw*)(kp + 16 * u));
+            v[u] = __builtin_bit_cast(Frag<T>, *(const Raw*)(vp + 16 * u));
+        }
+    }
+    // queries that see any of the keys: j0 - right .. j0 + 127 + left, to the end for a first token
+    const int lo = (int)max((int64_t)0, (int64_t)j0 - p.right) / TILE;
+    const int hi = j0 < p.sinks ? (p.S - 1) / TILE : (int)(min((int64_t)p.S - 1, (int64_t)j0 + KEYS - 1 + p.left) / TILE);
+    const int per = hi - lo + 1;
+    const int t0 = (int)((int64_t)G * per * cut / n), t1 = (int)((int64_t)G * per * (cut + 1) / n);
+    const float c = p.scale * LOG2E;
+    f32x16 dk[ND] = {}, dv[ND] = {};
+    Stage<D, TILE> sq, sg;
+    float se = 0.0f, sd = 0.0f;
+    const auto load = [&](int t) __attribute__((always_inline)) {
+        const int h = hk * G + t / per, q0 = (lo + t % per) * TILE;
+        sq.load((const uint16_t*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, q0, p.S - 1);
+        sg.load((const uint16_t*)p.dout + b * p.do_sb + h * p.do_sh, p.do_ss, q0, p.S - 1);
+        if (threadIdx.x < TILE) {
+            const int i = q0 + threadIdx.x;
+            const int64_t at = ((int64_t)b * p.H + h) * p.S + min(i, p.S - 1);
+            se = i < p.S ? lse2_of(p.lse[at]) : INFINITY;
+            sd = i < p.S ? delta[at] : 0.0f;
+        }
+    };
+    const auto store = [&](int t, int buf) __attribute__((always_inline)) {
+        const int left = p.S - (lo + t % per) * TILE;
+        const uint64_t rows = left >= 64 ? ~0ull : (1ull << left) - 1;
+        sq.store(lq[buf], rows);
+        sg.store(lg[buf], rows);
+        if (threadIdx.x < TILE) {
+            ls[buf][threadIdx.x] = se;
+            ld[buf][threadIdx.x] = sd;
+        }
+    };
+    if (t0 < t1) {
+        load(t0);
+        store(t0, 0);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1;
+        if (t + 1 < t1) load(t + 1);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int q0 = (lo + t % per) * TILE + 32 * u;
+            if (any == 0 || q0 >= p.S || none_seen(p, q0, jw, jw + 31)) continue;
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x) {
+                s = mfma(rows_frag<T, D>(lq[buf], 32 * u, x, lane), k[x], s);
+                dp = mfma(rows_frag<T, D>(lg[buf], 32 * u, x, lane), v[x], dp);
+            }
+            const bool cutoff = !all_seen(p, q0, jw, jw + 31);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 e = *(const f32x4*)&ls[buf][32 * u + 8 * g + 4 * (lane / 32)];
+                const f32x4 d = *(const f32x4*)&ld[buf][32 * u + 8 * g + 4 * (lane / 32)];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float w = exp2_(__builtin_fmaf(s[4 * g + r], c, -e[r]));
+                    if (cutoff) w = seen(p, q0 + row_of(4 * g + r, lane), j) ? w : 0.0f;
+                    s[4 * g + r] = w;
+                    dp[4 * g + r] = w * (dp[4 * g + r] - d[r]);
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const Frag<T> pf = round_frag<T>(s, w), df = round_frag<T>(dp, w);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    dv[d] = mfma(cols_frag<T, D>(lg[buf], 32 * u + 16 * w, 32 * d, lane), pf, dv[d]);
+                    dk[d] = mfma(cols_frag<T, D>(lq[buf], 32 * u + 16 * w, 32 * d, lane), df, dk[d]);
+                }
+            }
+        }
+        if (t + 1 < t1) store(t + 1, buf ^ 1);
+        __syncthreads();
+    }
+    if (j >= p.S) return;
+    if (n > 1) {                               // part[problem and item][dk, dv][key][D]
+        float* o = part + (int64_t)id * 2 * KEYS * D + (int64_t)(j - j0) * D + 4 * (lane / 32);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                f32x4 x, y;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = on ? dk[d][4 * g + r] * p.scale : 0.0f;
+                    y[r] = on ? dv[d][4 * g + r] : 0.0f;
+                }
+                *(f32x4*)(o + 32 * d + 8 * g) = x;
+                *(f32x4*)(o + KEYS * D + 32 * d + 8 * g) = y;
+            }
+        return;
+    }
+    const int64_t at = (((int64_t)b * p.S + j) * p.HK + hk) * D + 4 * (lane / 32);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float x[4], y[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                x[r] = on ? dk[d][4 * g + r] * p.scale : 0.0f;
+                y[r] = on ? dv[d][4 * g + r] : 0.0f;
+            }
+            store_n<T, 4>((T*)p.dk + at + 32 * d + 8 * g, 4, x);
+            store_n<T, 4>((T*)p.dv + at + 32 * d + 8 * g, 4, y);
+        }
+}
+
+// dk and dv of the split tiles: the float32 parts summed in order, four values a thread
+template <class T, int D>
+__global__ __launch_bounds__(NT) void k_attn_join(D8sAttnArgs p, const float* part, KeySplit ks) {
+    constexpr int KEYS = 128;
+    const int nk = (p.S + KEYS - 1) / KEYS, items = ks.sink_tiles * ks.sink_split + (nk - ks.sink_tiles) * ks.split;
+    const int joined = ks.split > 1 ? nk : ks.sink_tiles;          // tiles per problem, the first ones
+    const int kt = blockIdx.x % joined, bh = blockIdx.x / joined, b = bh / p.HK, hk = bh % p.HK;
+    const bool sink = kt < ks.sink_tiles;
+    const int n = sink ? ks.sink_split : ks.split;
+    const int first = sink ? kt * n : ks.sink_tiles * ks.sink_split + (kt - ks.sink_tiles) * n;
+    const float* src = part + ((int64_t)bh * items + first) * 2 * KEYS * D;
+    if (n == 1) return;                        // (written by its one workgroup)
+    const int e = (blockIdx.y * NT + threadIdx.x) * 4, which = e / (KEYS * D), j = kt * KEYS + e % (KEYS * D) / D;
+    if (j >= p.S) return;
+    f32x4 s = {};
+    for (int i = 0; i < n; ++i) s += *(const f32x4*)(src + (int64_t)i * 2 * KEYS * D + e);
+    T* o = (T*)(which ? p.dv : p.dk) + (((int64_t)b * p.S + j) * p.HK + hk) * D + e % D;
+    const float f[4] = {s[0], s[1], s[2], s[3]};
+    store_n<T, 4>(o, 4, f);
+}
+
+KeySplit key_split(const D8sAttnArgs* a) {
+    const int64_t S = a->S, nk = (S + 127) / 128, nq = (S + 63) / 64, G = a->H / a->HK;
+    const int64_t seen = std::min(nq, (std::min<int64_t>(a->left, S) + std::min<int64_t>(a->right, S) + 128) / 64 + 1);
+    const int64_t cus = d8s_host_cu_count(), problems = (int64_t)a->B * a->HK;
+    KeySplit k;
+    k.split = (int)std::max<int64_t>(1, std::min(cus / std::max<int64_t>(1, problems * nk), G * seen / 4));
+    k.sink_tiles = (int)std::min(nk, ((int64_t)a->sinks + 127) / 128);
+    k.sink_split = (int)std::min<int64_t>(G * nq, (k.split * nq + seen - 1) / seen);
+    return k;
+}
+int64_t key_items(const D8sAttnArgs* a, const KeySplit& k) {
+    const int64_t nk = (a->S + 127) / 128;
+    return (int64_t)k.sink_tiles * k.sink_split + (nk - k.sink_tiles) * k.split;
+}
+uint64_t delta_bytes(const D8sAttnArgs* a) { return ((uint64_t)a->B * a->H * a->S * 4 + 255) / 256 * 256; }
+
+// ---- one new token against a cache ------------------------------------------------------------------
+// A workgroup runs GM query heads of a key head over a share of the keys their token sees.  A key's row is read 16
+// bytes a lane by D / 8 lanes, so a wave reads 8 (D = 64) or 4 rows at a time; each group of lanes keeps the softmax
+// statistics and the sums of its own keys, and they are joined at the end, across the groups, the waves, and (k_join)
+// the shares.  Bound by memory: every key and value is read once for all the heads that share it (up to 8).
+template <class T, int D, int GM>
+__global__ __launch_bounds__(NT) void k_token(D8sTokenArgs p, int split, float* part) {
+    constexpr int LK = D / 8, KW = 64 / LK, U = 4;
+    __shared__ float sm[4][GM], sl[4][GM];
+    __shared__ float so[4][GM][D];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, gl = lane / LK, dl = lane % LK * 8;
+    const int G = p.H / p.HK, ng = (G + GM - 1) / GM;
+    const int cut = blockIdx.x % split, pr = blockIdx.x / split, g0 = pr % ng * GM, hk = pr / ng % p.HK, b = pr / ng / p.HK;
+    const int gn = min(GM, G - g0);
+    const int len = max(0, min(p.lengths[b], p.S)), lo = max(0, len - 1 - p.left), first = min(p.sinks, lo);
+    const int seen = first + len - lo;         // visible keys, the first tokens before the window's
+    const int e0 = (int)((int64_t)seen * cut / split), e1 = (int)((int64_t)seen * (cut + 1) / split);
+    const float c = p.scale * LOG2E;
+    float q[GM][8], acc[GM][8], m[GM], l[GM];
+#pragma unroll
+    for (int g = 0; g < GM; ++g) {
+        const int h = hk * G + g0 + min(g, gn - 1);
+        load_n<T, 8>((const T*)p.q + b * p.q_sb + h * p.q_sh + dl, 8, q[g]);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            q[g][d] *= c;
+            acc[g][d] = 0.0f;
+        }
+        m[g] = -INFINITY;
+        l[g] = 0.0f;
+    }
+    const T* kp = (const T*)p.k + b * p.k_sb + hk * p.k_sh + dl;
+    const T* vp = (const T*)p.v + b * p.v_sb + hk * p.v_sh + dl;
+    for (int e = e0 + wave * U * KW; e < e1; e += 4 * U * KW) {
+        Vec<T, 8> k[U], v[U];
+        bool on[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int x = e + u * KW + gl, xc = min(x, e1 - 1);
+            on[u] = x < e1;
+            const int64_t j = xc < first ? xc : lo + xc - first;
+            k[u] = *(const Vec<T, 8>*)(kp + j * p.k_ss);
+            v[u] = *(const Vec<T, 8>*)(vp + j * p.v_ss);
+        }
+#pragma unroll
+        for (int g = 0; g < GM; ++g) {
+            float s[U], top = m[g];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float x = 0.0f;
+#pragma unroll
+                for (int d = 0; d < 8; ++d) x = __builtin_fmaf(q[g][d], (float)k[u][d], x);
+                x = lanes_sum<LK>(x);
+                s[u] = on[u] ? x : -INFINITY;
+                top = fmaxf(top, s[u]);
+            }
+            const float base = top == -INFINITY ? 0.0f : top, a = exp2_(m[g] - base);
+            m[g] = top;
+            l[g] *= a;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) acc[g][d] *= a;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float w = exp2_(s[u] - base);
+                l[g] += w;
+                // (the row read in place of one past the end is a visible key's: its weight is 0, its values may not be)
+#pragma unroll
+                for (int d = 0; d < 8; ++d) acc[g][d] = on[u] ? __builtin_fmaf(w, (float)v[u][d], acc[g][d]) : acc[g][d];
+            }
+        }
+    }
+#pragma unroll
+    for (int g = 0; g < GM; ++g) {
+        float top = m[g], x, y;
+        if constexpr (LK == 8) top = fmaxf(top, dpp<0x128>(top));
+        swap16(top, x, y);
+        top = fmaxf(x, y);
+        swap32(top, x, y);
+        top = fmaxf(x, y);
+        const float a = top == -INFINITY ? 0.0f : exp2_(m[g] - top);
+        const auto join = [&](float f) __attribute__((always_inline)) {
+            f *= a;
+            if constexpr (LK == 8) f += dpp<0x128>(f);
+            swap16(f, x, y);
+            f = x + y;
+            swap32(f, x, y);
+            return x + y;
+        };
+        l[g] = join(l[g]);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) acc[g][d] = join(acc[g][d]);
+        if (gl == 0) {
+            if (dl == 0) {
+                sm[wave][g] = top;
+                sl[wave][g] = l[g];
+            }
+#pragma unroll
+            for (int d = 0; d < 8; ++d) so[wave][g][dl + d] = acc[g][d];
+        }
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < gn * D; x += NT) {
+        const int g = x / D, d = x % D;
+        const float top = fmaxf(fmaxf(sm[0][g], sm[1][g]), fmaxf(sm[2][g], sm[3][g]));
+        float o = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float a = sm[w][g] == -INFINITY ? 0.0f : exp2_(sm[w][g] - top);
+            o = __builtin_fmaf(so[w][g][d], a, o);
+            sum = __builtin_fmaf(sl[w][g], a, sum);
+        }
+        const int64_t head = (int64_t)b * p.H + hk * G + g0 + g;
+        if (split == 1) {
+            ((T*)p.out)[head * D + d] = (T)(len > 0 ? o / sum : 0.0f);
+        } else {                               // part[share][head][m, l, o ...]
+            float* t = part + ((int64_t)cut * p.B * p.H + head) * (D + 2);
+            if (d == 0) {
+                t[0] = top;
+                t[1] = sum;
+            }
+            t[2 + d] = o;
+        }
+    }
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(D) void k_join(const float* part, T* out, int split, int heads) {
+    const int head = blockIdx.x, d = threadIdx.x;
+    float top = -INFINITY, o = 0.0f, sum = 0.0f;
+    for (int s = 0; s < split; ++s) top = fmaxf(top, part[((int64_t)s * heads + head) * (D + 2)]);
+    for (int s = 0; s < split; ++s) {
+        const float* t = part + ((int64_t)s * heads + head) * (D + 2);
+        const float a = t[0] == -INFINITY ? 0.0f : exp2_(t[0] - top);
+        sum = __builtin_fmaf(t[1], a, sum);
+        o = __builtin_fmaf(t[2 + d], a, o);
+    }
+    out[(int64_t)head * D + d] = (T)(sum > 0.0f || sum != sum ? o / sum : 0.0f);
+}
+
+// Shares of a token's keys: enough workgroups for two a compute unit, at least 64 keys each
+int token_split(const D8sTokenArgs* a) {
+    const int G = a->H / a->HK, gm = G >= 8 ? 8 : G > 4 ? 8 : G > 2 ? 4 : G;
+    const int64_t problems = (int64_t)a->B * a->HK * ((G + gm - 1) / gm);
+    const int64_t seen = std::min<int64_t>(a->S, (int64_t)a->left + 1 + a->sinks);
+    return (int)std::max<int64_t>(1, std::min((2 * d8s_host_cu_count() + problems - 1) / problems, seen / 64));
+}
+
+template <class T, int D>
+void token_run(const D8sTokenArgs& a, hipStream_t st) {
+    const int G = a.H / a.HK, split = token_split(&a);
+    float* part = (float*)a.workspace;
+    const auto go = [&](auto kernel, int gm) {
+        const int64_t blocks = (int64_t)a.B * a.HK * ((G + gm - 1) / gm) * split;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(NT), 0, st, a, split, part);
+    };
+    if (G == 1) go(k_token<T, D, 1>, 1);
+    else if (G == 2) go(k_token<T, D, 2>, 2);
+    else if (G <= 4) go(k_token<T, D, 4>, 4);
+    else go(k_token<T, D, 8>, 8);
+    if (split > 1)
+        hipLaunchKernelGGL((k_join<T, D>), dim3((unsigned)(a.B * a.H)), dim3(D), 0, st, part, (T*)a.out, split, a.B * a.H);
+}
+
+template <class T, int D>
+void attn_run(const D8sAttnArgs& a, hipStream_t st) {
+    const unsigned grid = (unsigned)((int64_t)a.B * a.H * ((a.S + 127) / 128));
+    hipLaunchKernelGGL((k_attn<T, D>), dim3(grid), dim3(NT), 0, st, a);
+}
+
+template <class T, int D>
+void attn_back_run(const D8sAttnArgs& a, hipStream_t st) {
+    float* delta = (float*)a.workspace;
+    float* part = (float*)((char*)a.workspace + delta_bytes(&a));
+    const KeySplit ks = key_split(&a);
+    const unsigned grid = (unsigned)((int64_t)a.B * a.H * ((a.S + 127) / 128));
+    const int problems = a.B * a.HK, nk = (a.S + 127) / 128, joined = ks.split > 1 ? nk : ks.sink_split > 1 ? ks.sink_tiles : 0;
+    hipLaunchKernelGGL((k_attn_dq<T, D>), dim3(grid), dim3(NT), 0, st, a, delta);
+    hipLaunchKernelGGL((k_attn_dkv<T, D>), dim3((unsigned)(problems * key_items(&a, ks))), dim3(NT), 0, st, a, delta, part, ks);
+    if (joined)
+        hipLaunchKernelGGL((k_attn_join<T, D>), dim3((unsigned)(problems * joined), 2 * 128 * D / (4 * NT)), dim3(NT), 0, st,
+                           a, part, ks);
+}
+
+#define BY_TYPE(run, a, st)                                                                            \
+    do {                                                                                               \
+        if ((a).dtype == D8S_BF16) (a).D == 64 ? run<bf16, 64>((a), st) : run<bf16, 128>((a), st);     \
+        else (a).D == 64 ? run<f16, 64>((a), st) : run<f16, 128>((a), st);                             \
+    } while (0)
+
+int attn_check(const D8sAttnArgs* a, const char* what) {
+    AREQ(a != nullptr, "null arguments");
+    AREQ(a->dtype == D8S_BF16 || a->dtype == D8S_F16, "dtype must be D8S_BF16 or D8S_F16");
+    AREQ(a->D == 64 || a->D == 128, "D must be 64 or 128");
+    AREQ(a->B >= 1 && a->S >= 1 && a->H >= 1 && a->HK >= 1 && a->H % a->HK == 0, "bad sizes (H a multiple of HK)");
+    AREQ(a->S <= (1 << 30), "more than 2^30 tokens");
+    AREQ((int64_t)a->B * a->H * ((a->S + 127) / 128) < (1 << 24), "too many heads and tokens");
+    AREQ(a->left >= 0 && a->right >= 0 && a->sinks >= 0, "left, right and sinks must not be negative");
+    AREQ(a->scale > 0 && a->scale < INFINITY, "scale must be positive and finite");
+    AREQ(a->q && a->k && a->v && a->out, "null pointer");
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int d8s_attention(const D8sAttnArgs* a, void* stream) {
+    const char* what = "d8s_attention";
+    if (int rc = attn_check(a, what)) return rc;
+    BY_TYPE(attn_run, *a, (hipStream_t)stream);
+    return d8s_host_launched(what);
+}
+
+extern "C" int d8s_attention_workspace(const D8sAttnArgs* a, uint64_t* bytes) {
+    const char* what = "d8s_attention_workspace";
+    if (int rc = attn_check(a, what)) return rc;
+    AREQ(bytes != nullptr, "null arguments");
+    const KeySplit k = key_split(a);
+    const bool parts = k.split > 1 || (k.sink_tiles > 0 && k.sink_split > 1);
+    *bytes = delta_bytes(a) + (parts ? (uint64_t)a->B * a->HK * key_items(a, k) * 2 * 128 * a->D * 4 : 0);
+    return 0;
+}
+
+extern "C" int d8s_attention_backward(const D8sAttnArgs* a, void* stream) {
+    const char* what = "d8s_attention_backward";
+    if (int rc = attn_check(a, what)) return rc;
+    AREQ(a->lse && a->dout && a->dq && a->dk && a->dv && a->workspace, "null pointer");
+    uint64_t need = 0;
+    if (int rc = d8s_attention_workspace(a, &need)) return rc;
+    AREQ(a->ws_bytes >= need && ((uintptr_t)a->workspace & 15) == 0,
+         "workspace smaller than d8s_attention_workspace() or not 16-byte aligned");
+    AREQ((int64_t)a->B * a->HK * key_items(a, key_split(a)) < (1 << 24), "too many heads and tokens");
+    BY_TYPE(attn_back_run, *a, (hipStream_t)stream);
+    return d8s_host_launched(what);
+}
+
+static int token_check(const D8sTokenArgs* a, const char* what) {
+    AREQ(a != nullptr, "null arguments");
+    AREQ(a->dtype == D8S_BF16 || a->dtype == D8S_F16, "dtype must be D8S_BF16 or D8S_F16");
+    AREQ(a->D == 64 || a->D == 128, "D must be 64 or 128");
+    AREQ(a->B >= 1 && a->S >= 1 && a->H >= 1 && a->HK >= 1 && a->H % a->HK == 0, "bad sizes (H a multiple of HK)");
+    AREQ((int64_t)a->B * a->H < (1 << 22), "too many heads");
+    AREQ(a->left >= 0 && a->sinks >= 0, "left and sinks must not be negative");
+    AREQ(a->scale > 0 && a->scale < INFINITY, "scale must be positive and finite");
+    return 0;
+}
+
+extern "C" int d8s_attention_token_workspace(const D8sTokenArgs* a, uint64_t* bytes) {
+    const char* what = "d8s_attention_token_workspace";
+    if (int rc = token_check(a, what)) return rc;
+    AREQ(bytes != nullptr, "null arguments");
+    const int split = token_split(a);
+    *bytes = split > 1 ? (uint64_t)split * a->B * a->H * (a->D + 2) * 4 : 0;
+    return 0;
+}
+
+extern "C" int d8s_attention_token(const D8sTokenArgs* a, void* stream) {
+    const char* what = "d8s_attention_token";
+    if (int rc = token_check(a, what)) return rc;
+    AREQ(a->q && a->k && a->v && a->out && a->lengths, "null pointer");
+    uint64_t need = 0;
+    if (int rc = d8s_attention_token_workspace(a, &need)) return rc;
+    AREQ(need == 0 || (a->workspace && a->ws_bytes >= need), "workspace smaller than d8s_attention_token_workspace()");
+    BY_TYPE(token_run, *a, (hipStream_t)stream);
+    return d8s_host_launched(what);
+}

@@ -24,7 +24,8 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 SOURCE = CSRC / "d8s_kernels.hip"
 # every file compiled into the library (the first is SOURCE)
-SOURCES = (SOURCE, CSRC / "d8s_prep.hip", CSRC / "d8s_head.hip", CSRC / "d8s_host.h")
+SOURCES = (SOURCE, CSRC / "d8s_prep.hip", CSRC / "d8s_head.hip", CSRC / "d8s_context.hip",
+           CSRC / "d8s_attention.hip", CSRC / "d8s_optim.hip", CSRC / "d8s_elem.h", CSRC / "d8s_host.h")
 HEADER = PKG.parent / "include" / "d8s_hip.h"
 LIB_PATH = PKG / "libd8s_hip.so"
 ABI_VERSION = 1
@@ -41,7 +42,7 @@ class D8sError(RuntimeError):
         self.code = code
 
 
-i32, u64, vp = ctypes.c_int32, ctypes.c_uint64, ctypes.c_void_p
+i32, i64, u64, vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64, ctypes.c_void_p
 
 
 class GemmArgs(ctypes.Structure):
@@ -149,6 +150,61 @@ class HeadArgs(ctypes.Structure):
                 + [(n, i32) for n in ("B", "W", "D", "S", "CD", "heads", "FF", "PER", "T", "ctx_layers")])
 
 
+class NormArgs(ctypes.Structure):
+    """`D8sNormArgs`: layer norm and its gradients."""
+    _fields_ = ([(n, u64) for n in ("x", "w", "b", "y", "mean", "rstd", "dy", "dx", "dw", "db", "partial",
+                                    "partial_bytes")]
+                + [(n, i64) for n in ("rows", "x_stride", "dy_stride")]
+                + [("width", i32), ("dtype", i32), ("wdtype", i32), ("eps", ctypes.c_float)])
+
+
+ROTARY_PAIRS = 256                       # `D8S_ROTARY_PAIRS`
+
+
+class RotaryArgs(ctypes.Structure):
+    """`D8sRotaryArgs`: rotary positions of several axes."""
+    _fields_ = ([("x", u64), ("y", u64), ("pos", u64)]
+                + [(n, i64) for n in ("x_sb", "x_ss", "x_sh", "y_sb", "y_ss", "y_sh", "pos_sb", "pos_ss")]
+                + [(n, i32) for n in ("B", "S", "H", "D", "pairs", "axes", "dtype", "pos_type", "adjacent", "inverse")]
+                + [("freq", ctypes.c_double * ROTARY_PAIRS), ("axis", ctypes.c_uint8 * ROTARY_PAIRS)])
+
+
+class AttnArgs(ctypes.Structure):
+    """`D8sAttnArgs`: attention within a window and first tokens, and its gradients."""
+    _fields_ = ([(n, u64) for n in ("q", "k", "v", "mask", "out", "lse", "dout", "dq", "dk", "dv", "workspace",
+                                    "ws_bytes")]
+                + [(n, i64) for n in ("q_sb", "q_ss", "q_sh", "k_sb", "k_ss", "k_sh", "v_sb", "v_ss", "v_sh",
+                                      "do_sb", "do_ss", "do_sh", "mask_sb")]
+                + [(n, i32) for n in ("B", "S", "H", "HK", "D", "dtype", "left", "right", "sinks")]
+                + [("scale", ctypes.c_float)])
+
+
+class TokenArgs(ctypes.Structure):
+    """`D8sTokenArgs`: attention of one new token a row against a cache."""
+    _fields_ = ([(n, u64) for n in ("q", "k", "v", "lengths", "out", "workspace", "ws_bytes")]
+                + [(n, i64) for n in ("q_sb", "q_sh", "k_sb", "k_ss", "k_sh", "v_sb", "v_ss", "v_sh")]
+                + [(n, i32) for n in ("B", "S", "H", "HK", "D", "dtype", "left", "sinks")]
+                + [("scale", ctypes.c_float), ("pad_", i32)])
+
+
+ADAMW_BLOCK = 256                        # `D8S_ADAMW_BLOCK`
+
+
+class AdamwTensor(ctypes.Structure):
+    """`D8sAdamwTensor`: one parameter tensor of a step."""
+    _fields_ = [("p", u64), ("g", u64), ("n", i64), ("at", i64)]
+
+
+class AdamwArgs(ctypes.Structure):
+    """`D8sAdamwArgs`: an AdamW step over many tensors."""
+    _fields_ = ([(n, u64) for n in ("tensors", "m", "v", "m_scale", "v_scale", "grad_scale")] + [("step", i64)]
+                + [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+                + [(n, i32) for n in ("count", "dtype", "grad_dtype", "bits")])
+
+
+# element types of the context layer's and the optimizer's tensors (`D8S_F32`, `D8S_BF16`, `D8S_F16`)
+ELEMENTS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
 IN_F16, IN_U8 = 0, 1
 
 # entry point -> argument types (all return int32 status)
@@ -189,6 +245,17 @@ SIGNATURES = {
     "d8s_head_workspace": [ctypes.POINTER(HeadArgs), ctypes.POINTER(ctypes.c_uint64)],
     "d8s_head": [ctypes.POINTER(HeadArgs), vp],
     "d8s_head_noalloc": [ctypes.POINTER(HeadArgs), vp],
+    "d8s_layer_norm": [ctypes.POINTER(NormArgs), vp],
+    "d8s_layer_norm_workspace": [ctypes.POINTER(NormArgs), ctypes.POINTER(ctypes.c_uint64)],
+    "d8s_layer_norm_backward": [ctypes.POINTER(NormArgs), vp],
+    "d8s_rotary": [ctypes.POINTER(RotaryArgs), vp],
+    "d8s_attention": [ctypes.POINTER(AttnArgs), vp],
+    "d8s_attention_workspace": [ctypes.POINTER(AttnArgs), ctypes.POINTER(ctypes.c_uint64)],
+    "d8s_attention_backward": [ctypes.POINTER(AttnArgs), vp],
+    "d8s_attention_token": [ctypes.POINTER(TokenArgs), vp],
+    "d8s_attention_token_workspace": [ctypes.POINTER(TokenArgs), ctypes.POINTER(ctypes.c_uint64)],
+    "d8s_adamw": [ctypes.POINTER(AdamwArgs), vp],
+    "d8s_adamw_moments": [vp, vp, vp, vp, i64, vp, vp, vp],
     "d8s_micro_copy": [vp, vp, ctypes.c_size_t, vp],
     "d8s_micro_mfma": [i32, i32, vp, vp],
     "d8s_probe_mfma_i8": [vp, vp, vp, vp],

@@ -1,0 +1,150 @@
+"""AdamW over many tensors at once on the GPU (`d8s_adamw`, include/d8s_hip.h): the optimizer that trains a head or a
+context layer, with moments in 32 or 8 bits.
+
+    opt = AdamW(model.parameters(), lr=1e-3, state_bits=8)
+    loss.backward()
+    opt.step()                           # or opt.step(grads), opt.step(grad_scale=scale on the GPU)
+
+A step is one launch for every 100 tensors of one pair of types, whatever their sizes.  There is no CPU path: without
+the library the calls raise.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import torch
+
+from . import hip
+
+_ROW = np.dtype([("p", "u8"), ("g", "u8"), ("n", "i8"), ("at", "i8")])       # AdamwTensor
+
+
+class AdamW:
+    """p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps) after
+    m = beta1 m + (1 - beta1) g and v = beta2 v + (1 - beta2) g^2, all in float32 with every operation rounded by
+    itself, p then to its type.
+
+    params: contiguous float32, bfloat16 or float16 tensors on one GPU; gradients are float32 or 16 bits beside
+    float32 parameters, float32 or the parameter's own type beside 16-bit ones.  The moments of all tensors lie in
+    one array each, tensor i's padded to whole blocks of 256 elements (the padding stays zeros).  state_bits 8 keeps
+    them as codes with one float32 scale a block, 2.03 bytes an element in place of 8: m = scale c |c| / 127^2 and
+    sqrt(v) = scale c^2 / 255^2.  Gradients must be finite: one that is not spoils its element, with state_bits 8
+    its block's moments."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
+                 state_bits: int = 32) -> None:
+        self.params = list(params)
+        if not self.params:
+            raise ValueError("no parameters")
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        if len({id(p) for p in self.params}) != len(self.params):
+            raise ValueError("a parameter is given twice")
+        if not (lr >= 0 and eps > 0 and weight_decay >= 0 and 0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+            raise ValueError("lr and weight_decay must not be negative, eps positive, betas in [0, 1)")
+        self.device = self.params[0].device
+        for p in self.params:
+            self._check(p)
+        self.lr, self.betas, self.eps, self.weight_decay, self.state_bits = lr, tuple(betas), eps, weight_decay, state_bits
+        self.step_count = 0
+        block = hip.ADAMW_BLOCK
+        self._table = np.zeros(len(self.params), _ROW)
+        self._table["n"] = [p.numel() for p in self.params]
+        padded = (self._table["n"] + block - 1) // block * block
+        self._table["at"] = np.cumsum(padded) - padded
+        total = max(block, int(padded.sum()))
+
+        def zeros(n, dtype):
+            return torch.zeros(n, dtype=dtype, device=self.device)
+        if state_bits == 8:
+            self._state = {"m_code": zeros(total, torch.int8), "v_code": zeros(total, torch.uint8),
+                           "m_scale": zeros(total // block, torch.float32), "v_scale": zeros(total // block, torch.float32)}
+        else:
+            self._state = {"m": zeros(total, torch.float32), "v": zeros(total, torch.float32)}
+        self._dtypes = [p.dtype for p in self.params]
+
+    def _check(self, p: torch.Tensor) -> None:
+        if p.dtype not in hip.ELEMENTS or not p.is_contiguous() or p.device != self.device or p.device.type != "cuda":
+            raise ValueError("parameters must be contiguous float32, bfloat16 or float16 tensors on one GPU")
+
+    def step(self, grads=None, grad_scale: torch.Tensor | None = None) -> None:
+        """One step in place.  grads: a tensor, or None, for every parameter (default: their .grad); parameters
+        without one are left as they are, their moments too.  grad_scale: one float32 on the GPU that every
+        gradient is multiplied by.  The step's numbers are arguments of its launches, so it cannot be recorded into
+        a graph."""
+        grads = [p.grad for p in self.params] if grads is None else list(grads)
+        if len(grads) != len(self.params):
+            raise ValueError("a gradient (or None) for every parameter is required")
+        stream = torch.cuda.current_stream(self.device)
+        if hip.capturing(stream):
+            raise RuntimeError("an optimizer step cannot be recorded into a graph")
+        if grad_scale is not None and (grad_scale.numel() != 1 or grad_scale.dtype != torch.float32
+                                       or grad_scale.device != self.device):
+            raise ValueError("grad_scale must be one float32 on the parameters' GPU")
+        kinds: dict[tuple, list[int]] = {}
+        kept = []                              # (copies live until the launches are enqueued)
+        for i, (p, g) in enumerate(zip(self.params, grads)):
+            if g is None:
+                continue
+            if g.shape != p.shape or g.device != self.device:
+                raise ValueError(f"gradient {i} must have its parameter's shape and device")
+            if p.dtype != self._dtypes[i] or p.numel() != self._table["n"][i] or not p.is_contiguous():
+                raise ValueError(f"parameter {i} has changed")
+            if g.dtype not in hip.ELEMENTS or not (g.dtype == p.dtype or torch.float32 in (g.dtype, p.dtype)):
+                raise ValueError(f"gradient {i}: {g.dtype} beside {p.dtype}")
+            if not g.is_contiguous():
+                g = g.contiguous()
+                kept.append(g)
+            kinds.setdefault((p.dtype, g.dtype), []).append(i)
+            self._table["p"][i], self._table["g"][i] = p.data_ptr(), g.data_ptr()
+        s = self._state
+        a = hip.AdamwArgs()
+        if self.state_bits == 8:
+            a.m, a.v, a.m_scale, a.v_scale = (s[n].data_ptr() for n in ("m_code", "v_code", "m_scale", "v_scale"))
+        else:
+            a.m, a.v = s["m"].data_ptr(), s["v"].data_ptr()
+        a.grad_scale = 0 if grad_scale is None else grad_scale.data_ptr()
+        a.step, a.bits = self.step_count + 1, self.state_bits
+        a.lr, a.beta1, a.beta2, a.eps, a.weight_decay = self.lr, *self.betas, self.eps, self.weight_decay
+        with torch.cuda.device(self.device):
+            for (pt, gt), which in kinds.items():
+                rows = self._table if len(which) == len(self.params) else self._table[which]
+                a.tensors, a.count = rows.ctypes.data, len(rows)
+                a.dtype, a.grad_dtype = hip.ELEMENTS[pt], hip.ELEMENTS[gt]
+                hip.call("d8s_adamw", ctypes.byref(a), ctypes.c_void_p(stream.cuda_stream))
+        self.step_count += 1
+        hip.written(*(self.params[i] for which in kinds.values() for i in which), *s.values())
+
+    def moments(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """Both moments of all tensors, (elements,) float32, laid out as the state is: the state's own arrays, or
+        new ones of the values that 8-bit moments stand for."""
+        s = self._state
+        if self.state_bits == 32:
+            return s["m"], s["v"]
+        m, v = (torch.empty(s["m_code"].numel(), dtype=torch.float32, device=self.device) for _ in range(2))
+        with torch.cuda.device(self.device):
+            hip.call("d8s_adamw_moments", *(s[n].data_ptr() for n in ("m_code", "v_code", "m_scale", "v_scale")),
+                     m.numel(), m.data_ptr(), v.data_ptr(), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        return m, v
+
+    def zero_grad(self) -> None:
+        for p in self.params:
+            p.grad = None
+
+    def state_dict(self) -> dict:
+        """The step count and copies of the moments as they are kept."""
+        return {"step": self.step_count, **{n: t.clone() for n, t in self._state.items()}}
+
+    def load_state_dict(self, state: dict) -> None:
+        """Takes over what `state_dict` gave of an optimizer over tensors of the same sizes and state_bits."""
+        if set(state) != {"step", *self._state}:
+            raise ValueError(f"the state must hold step and {sorted(self._state)}")
+        for n, t in self._state.items():
+            if state[n].shape != t.shape or state[n].dtype != t.dtype:
+                raise ValueError(f"{n} must be {tuple(t.shape)} {t.dtype}")
+        if int(state["step"]) < 0:
+            raise ValueError("step must not be negative")
+        for n, t in self._state.items():
+            t.copy_(state[n])
+        self.step_count = int(state["step"])
