@@ -51,7 +51,7 @@ def _oracle(q, k, v, dout, left, right, sinks, mask, scale):
     ds = p * (dp - row)
     erow = (u * (do * o).abs() + 2.0 ** -20 * (do * o).abs() + tiny * do.abs()).sum(-1, keepdim=True) + (do.abs() * e).sum(-1, keepdim=True)
     edp = 2 * d * 2.0 ** -24 * (do.abs() @ v.abs().transpose(2, 3))
-    eds = (u + 4 * es) * ds.abs() + p * (erow + edp) + tiny * see
+    eds = (u + 4 * es) * ds.abs() + p * (erow + edp) + (tiny + 2.0 ** -126 * (dp - row).abs()) * see
     dq, dk, dv = ds @ k * scale, ds.transpose(2, 3) @ q * scale, p.transpose(2, 3) @ do
     edq = eds @ k.abs() * scale + u * dq.abs() + tiny
     edk = eds.transpose(2, 3) @ q.abs() * scale
