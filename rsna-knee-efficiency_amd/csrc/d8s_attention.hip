@@ -92,87 +92,135 @@ DEV Frag<T> round_frag(const f32x16& x, int s) {
     return f;
 }
 
-DEV int row_of(int r, int lane) { return r % 4 + 8 * (r / 4) + 4 * (lane / 32); }
-
 // Consecutive problems on one XCD's L2: workgroup w runs problem (w % 8) (n / 8) + w / 8 (as far as 8 divides n)
 DEV int xcd_order(int w, int n) {
     const int per = n / 8;
     return w < 8 * per ? (w % 8) * per + w / 8 : w;
 }
 
-// The tiles of TILE keys a run of queries i0 .. i1 can see: the first tokens' ones, then the window's
+// The tiles of 64 keys a run of queries i0 .. i1 can see: the first tokens' ones, then the window's
+constexpr int TILE = 64;
 struct Tiles {
     int first, start, count;
     DEV int at(int i) const { return i < first ? i : start + i - first; }
 };
-template <int TILE>
 DEV Tiles tiles_of(const D8sAttnArgs& p, int i0, int i1) {
-    const int lo = max(0, i0 - p.left) / TILE, hi = min((int64_t)p.S - 1, (int64_t)i1 + p.right) / TILE;
-    const int first = min((min(p.sinks, p.S) + TILE - 1) / TILE, lo);
+    const int lo = max(0, i0 - p.left) / TILE, hi = min(p.S - 1, i1 + p.right) / TILE;
+    const int first = min((p.sinks + TILE - 1) / TILE, lo);
     return {first, lo, first + hi - lo + 1};
 }
 
-// Whether queries i0 .. i0 + 31 see none, or all, of keys k0 .. k1
+// Whether queries i0 .. i0 + 31 see none, or all, of keys k0 .. k1 (left, right and sinks are at most S, and S at
+// most 2^29: no sum of them overflows)
 DEV bool none_seen(const D8sAttnArgs& p, int i0, int k0, int k1) {
-    return k0 > (int64_t)i0 + 31 + p.right || (k1 < i0 - p.left && k0 >= p.sinks);
+    return k0 > i0 + 31 + p.right || (k1 < i0 - p.left && k0 >= p.sinks);
 }
 DEV bool all_seen(const D8sAttnArgs& p, int i0, int k0, int k1) {
-    return k1 <= (int64_t)i0 + p.right && (k0 >= i0 + 31 - p.left || k1 < p.sinks);
-}
-DEV bool seen(const D8sAttnArgs& p, int i, int j) {
-    return j <= (int64_t)i + p.right && (j >= i - p.left || j < p.sinks);
+    return k1 <= i0 + p.right && (k0 >= i0 + 31 - p.left || k1 < p.sinks);
 }
 
-// One thread's share of a tile of ROWS rows, in registers between memory and LDS
+// Bits 0 .. 63 below n, or from n on (any n)
+DEV uint64_t bits_below(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : ~(~0ull << n); }
+DEV uint64_t bits_from(int n) { return ~bits_below(n); }
+
+// What a lane keeps of its 16 registers of a 32 x 32 result whose row r is kept iff bit r of `rows` is set: the bits
+// moved so that register r's is at r % 4 + 8 (r / 4)
+DEV uint32_t lane_rows(uint32_t rows, int lane) { return rows >> (4 * (lane / 32)); }
+DEV uint32_t keep_mask(uint32_t lane_bits, int r) {       // all ones where register r is kept (one v_bfe_i32)
+    return (uint32_t)__builtin_amdgcn_sbfe((int)lane_bits, r % 4 + 8 * (r / 4), 1);
+}
+
+// Copies a tile of ROWS rows of a matrix (rows `stride` elements apart, those past `last` replaced by it) to LDS
+// without registers: each lane of a wave's copy brings the 16 bytes that belong at its place of the swizzled tile.
 template <int D, int ROWS>
-struct Stage {
-    static constexpr int N = ROWS * D / 8 / NT;
-    Raw v[N];
-    // rows r0 .. of a matrix whose rows are `stride` elements apart; rows past `last` are read as `last`
-    DEV void load(const uint16_t* p, int64_t stride, int r0, int last) {
+struct Copy {
+    static constexpr int P = D / 8, N = ROWS * P / NT, STEP = NT / P;   // rows between a thread's pieces
+    int row, col;                              // of the thread's first piece
+    DEV Copy() {
+        row = threadIdx.x / P;
+        col = 8 * (piece<D>(row, threadIdx.x % P) % P);    // (the swizzle is its own inverse, and repeats every STEP rows)
+        static_assert(STEP % 16 == 0, "swizzle");
+    }
+    DEV void operator()(const uint16_t* p, int64_t stride, int r0, int last, u32x4* tile, int wave) const {
+        typedef const __attribute__((address_space(1))) void* global;
+        typedef __attribute__((address_space(3))) void* lds;
+        if (r0 + ROWS - 1 <= last) {
+            const uint16_t* q = p + r0 * stride + (row * stride + col);
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int id = n * NT + threadIdx.x, r = min(r0 + id / (D / 8), last);
-            v[n] = *(const Raw*)(p + r * stride + id % (D / 8) * 8);
+            for (int n = 0; n < N; ++n)
+                __builtin_amdgcn_global_load_lds((global)(q + n * STEP * stride), (lds)(tile + n * NT + wave * 64), 16, 0, 0);
+        } else {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                __builtin_amdgcn_global_load_lds((global)(p + min(r0 + row + n * STEP, last) * stride + col),
+                                                 (lds)(tile + n * NT + wave * 64), 16, 0, 0);
         }
     }
-    // rows whose bit is not set become zeros (whatever memory holds there)
-    DEV void store(u32x4* tile, uint64_t bits) const {
+    // zeros in the thread's own pieces of rows whose bit is not set (its copies have arrived)
+    DEV void clear(u32x4* tile, uint64_t rows) const {
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int id = n * NT + threadIdx.x, r = id / (D / 8);
-            const u32x4 x = __builtin_bit_cast(u32x4, v[n]);
-            tile[piece<D>(r, id % (D / 8))] = bits >> r & 1 ? x : u32x4{0, 0, 0, 0};
-        }
+        for (int n = 0; n < N; ++n)
+            if (!(rows >> (row + n * STEP) & 1)) tile[n * NT + threadIdx.x] = u32x4{0, 0, 0, 0};
+    }
+};
+DEV void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Which of the tile's keys exist and are not masked, from the byte a lane read for its key
+struct KeyBits {
+    const uint8_t* mask;
+    int S;
+    uint8_t byte;
+    DEV void load(int k0, int lane) { byte = mask ? mask[min(k0 + lane, S - 1)] : 1; }
+    DEV uint64_t bits(int k0) const {
+        const uint64_t in = bits_below(S - k0);
+        return mask ? __ballot(byte != 0) & in : in;
     }
 };
 
-// Bit r: key k0 + r exists and is not masked
-DEV uint64_t key_bits(const uint8_t* mask, int S, int k0, int lane) {
-    const int k = k0 + lane;
-    const bool on = k < S && (mask == nullptr || mask[min(k, S - 1)] != 0);
-    return __ballot(on);
+// Rows of results held by lane columns (column l % 32, rows as in lane_rows): values 32 d + ... of row `o`, scaled,
+// rounded, and joined between the wave's halves into 16-byte stores.
+template <class T, int ND>
+DEV void store_rows(T* o, const f32x16* acc, float scale, bool on, int lane) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; g += 2) {
+            typedef T half4 __attribute__((ext_vector_type(4)));
+            u32x2 w[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                half4 h;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) h[j] = (T)(acc[d][4 * (g + k) + j] * scale);
+                w[k] = __builtin_bit_cast(u32x2, h);
+            }
+            const u32x2 a = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+            const u32x2 b = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+            // lower lanes: values 8 g .. 8 g + 7; upper lanes: the eight after them
+            const Vec<uint32_t, 4> v = {a[0], b[0], a[1], b[1]};
+            typedef Vec<uint16_t, 8> out8;
+            if (on) *(out8*)(o + 32 * d + 8 * (g + lane / 32)) = __builtin_bit_cast(out8, v);
+        }
 }
 
 // ---- forward --------------------------------------------------------------------------------------
 // A workgroup runs 128 queries of a head, 32 a wave, over the tiles of 64 keys they can see; keys and values go
-// through two LDS buffers, the next tile's loads in flight while one is computed.  A wave forms s transposed (keys x
+// through two LDS buffers, the next tile's copies in flight while one is computed.  A wave forms s transposed (keys x
 // queries), so a query's statistics are one value a lane, and P goes from registers into the second product.
 // The running maximum m is raised, and the sums scaled, only where a tile exceeds it by more than 2^RISE (P stays below
 // 2^RISE, harmless in float32 and in both types), which after a row's first tiles is rare.
 constexpr float RISE = 6.0f;
 
 template <class T, int D>
-__global__ __launch_bounds__(NT, 2) void k_attn(D8sAttnArgs p) {
-    constexpr int TILE = 64, ND = D / 32;
+__global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
+    constexpr int ND = D / 32;
     __shared__ u32x4 lk[2][TILE * D / 8], lv[2][TILE * D / 8];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int nq = (p.S + 127) / 128, id = xcd_order(blockIdx.x, gridDim.x);
     const int b = id / (nq * p.H), h = id / nq % p.H, i00 = id % nq * 128, i0 = i00 + 32 * wave;
     const int hk = h / (p.H / p.HK);
     const uint16_t* kp = (const uint16_t*)p.k + b * p.k_sb + hk * p.k_sh;
     const uint16_t* vp = (const uint16_t*)p.v + b * p.v_sb + hk * p.v_sh;
-    const uint8_t* mask = p.mask ? p.mask + b * p.mask_sb : nullptr;
     const int i = i0 + lane % 32;
     Frag<T> q[D / 16];
     {
@@ -184,98 +232,89 @@ __global__ __launch_bounds__(NT, 2) void k_attn(D8sAttnArgs p) {
     const float c = p.scale * LOG2E;
     float m = -INFINITY, l = 0.0f;
     f32x16 acc[ND] = {};
-    const Tiles tiles = tiles_of<TILE>(p, i00, min(i00 + 127, p.S - 1));
-    Stage<D, TILE> sk, sv;
+    const Tiles tiles = tiles_of(p, i00, min(i00 + 127, p.S - 1));
+    const Copy<D, TILE> copy;
+    KeyBits keys{p.mask ? p.mask + b * p.mask_sb : nullptr, p.S, 1};
     int k0 = tiles.at(0) * TILE;
-    uint64_t bits = key_bits(mask, p.S, k0, lane);
-    sk.load(kp, p.k_ss, k0, p.S - 1);
-    sv.load(vp, p.v_ss, k0, p.S - 1);
-    sk.store(lk[0], bits);
-    sv.store(lv[0], bits);
-    __syncthreads();
+    copy(kp, p.k_ss, k0, p.S - 1, lk[0], wave);
+    copy(vp, p.v_ss, k0, p.S - 1, lv[0], wave);
+    keys.load(k0, lane);
     for (int t = 0; t < tiles.count; ++t) {
-        uint64_t next = 0;
-        int k1 = 0;
-        if (t + 1 < tiles.count) {
-            k1 = tiles.at(t + 1) * TILE;
-            next = key_bits(mask, p.S, k1, lane);
-            sk.load(kp, p.k_ss, k1, p.S - 1);
-            sv.load(vp, p.v_ss, k1, p.S - 1);
+        u32x4 *tk = lk[t & 1], *tv = lv[t & 1];
+        arrived();
+        const uint64_t bits = keys.bits(k0);
+        if (bits != ~0ull) {                   // whatever memory holds of a masked key is not used
+            copy.clear(tk, bits);
+            copy.clear(tv, bits);
         }
-        if (bits != 0 && !none_seen(p, i0, k0, k0 + TILE - 1)) {
-            const u32x4 *tk = lk[t & 1], *tv = lv[t & 1];
-            f32x16 s[2] = {};
+        __syncthreads();                       // the tile is there, and the other one is no longer read
+        const int now = k0;
+        if (t + 1 < tiles.count) {
+            k0 = tiles.at(t + 1) * TILE;
+            copy(kp, p.k_ss, k0, p.S - 1, lk[(t + 1) & 1], wave);
+            copy(vp, p.v_ss, k0, p.S - 1, lv[(t + 1) & 1], wave);
+            keys.load(k0, lane);
+        }
+        if (bits == 0 || none_seen(p, i0, now, now + TILE - 1)) continue;
+        f32x16 s[2];
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k)
+        for (int u = 0; u < 2; ++u) {
+            s[u] = mfma(rows_frag<T, D>(tk, 32 * u, 0, lane), q[0], f32x16{});
 #pragma unroll
-                for (int u = 0; u < 2; ++u) s[u] = mfma(rows_frag<T, D>(tk, 32 * u, k, lane), q[k], s[u]);
-            if (bits != ~0ull || !all_seen(p, i0, k0, k0 + TILE - 1)) {
+            for (int k = 1; k < D / 16; ++k) s[u] = mfma(rows_frag<T, D>(tk, 32 * u, k, lane), q[k], s[u]);
+        }
+        if (bits != ~0ull || !all_seen(p, i0, now, now + TILE - 1)) {
+            const uint64_t vis = bits & bits_below(i + p.right + 1 - now) & (bits_from(i - p.left - now) | bits_below(p.sinks - now));
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int j = 32 * u + row_of(r, lane);
-                        s[u][r] = (bits >> j & 1) && seen(p, i, k0 + j) ? s[u][r] : -INFINITY;
-                    }
-            }
-            float top = s[0][0];
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-            float t0, t1;
-            swap32(top, t0, t1);
-            top = fmaxf(t0, t1);
-            if (__any(top * c > m * c + RISE)) {
-                const float up = fmaxf(m, top), a = up == -INFINITY ? 1.0f : exp2_((m - up) * c);
-                m = up;
-                l *= a;
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[d][r] *= a;
-            }
-            const float mc = m == -INFINITY ? 0.0f : m * c;
-            float sum = 0.0f;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t mine = lane_rows((uint32_t)(vis >> (32 * u)), lane);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    s[u][r] = exp2_(__builtin_fmaf(s[u][r], c, -mc));
-                    sum += s[u][r];
+                    const uint32_t keep = keep_mask(mine, r);
+                    s[u][r] = __uint_as_float((__float_as_uint(s[u][r]) & keep) | (0xff800000u & ~keep));
                 }
-            l += sum;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const Frag<T> w = round_frag<T>(s[u / 2], u % 2);
-#pragma unroll
-                for (int d = 0; d < ND; ++d) acc[d] = mfma(cols_frag<T, D>(tv, 16 * u, 32 * d, lane), w, acc[d]);
             }
         }
-        if (t + 1 < tiles.count) {
-            sk.store(lk[(t + 1) & 1], next);
-            sv.store(lv[(t + 1) & 1], next);
+        float top = s[0][0];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+        float t0, t1;
+        swap32(top, t0, t1);
+        top = fmaxf(t0, t1);
+        if (__any(top * c > m * c + RISE)) {
+            const float up = fmaxf(m, top), a = up == -INFINITY ? 1.0f : exp2_((m - up) * c);
+            m = up;
+            l *= a;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[d][r] *= a;
         }
-        bits = next;
-        k0 = k1;
-        __syncthreads();
+        const float mc = m == -INFINITY ? 0.0f : m * c;
+        float sum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[u][r] = exp2_(__builtin_fmaf(s[u][r], c, -mc));
+                sum += s[u][r];
+            }
+        l += sum;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const Frag<T> w = round_frag<T>(s[u / 2], u % 2);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) acc[d] = mfma(cols_frag<T, D>(tv, 16 * u, 32 * d, lane), w, acc[d]);
+        }
     }
     float l0, l1;
     swap32(l, l0, l1);
     l = l0 + l1;
-    if (i >= p.S) return;
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    if (p.lse && lane < 32) p.lse[((int64_t)b * p.H + h) * p.S + i] = l > 0.0f || l != l ? (m * c + log2f(l)) * LN2 : -INFINITY;
-    T* o = (T*)p.out + (((int64_t)b * p.S + i) * p.H + h) * D + 4 * (lane / 32);
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            float f[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) f[j] = acc[d][4 * g + j] * inv;
-            store_n<T, 4>(o + 32 * d + 8 * g, 4, f);
-        }
+    const bool any = l > 0.0f || l != l;       // (a sum that is not a number stays one)
+    if (p.lse && lane < 32 && i < p.S) p.lse[((int64_t)b * p.H + h) * p.S + i] = any ? (m * c + log2f(l)) * LN2 : -INFINITY;
+    store_rows<T, ND>((T*)p.out + (((int64_t)b * p.S + i) * p.H + h) * D, acc, any ? 1.0f / l : 0.0f, i < p.S, lane);
 }
 
 // ---- backward: queries ------------------------------------------------------------------------------
@@ -284,17 +323,17 @@ __global__ __launch_bounds__(NT, 2) void k_attn(D8sAttnArgs p) {
 DEV float lse2_of(float lse) { return lse == -INFINITY ? INFINITY : lse * LOG2E; }   // (empty row: every P is 0)
 
 template <class T, int D>
-__global__ __launch_bounds__(NT, 2) void k_attn_dq(D8sAttnArgs p, float* delta) {
-    constexpr int TILE = 64, ND = D / 32;
+__global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn_dq(D8sAttnArgs p, float* delta) {
+    constexpr int ND = D / 32;
     __shared__ u32x4 lk[2][TILE * D / 8], lv[2][TILE * D / 8];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int nq = (p.S + 127) / 128, id = xcd_order(blockIdx.x, gridDim.x);
     const int b = id / (nq * p.H), h = id / nq % p.H, i00 = id % nq * 128, i0 = i00 + 32 * wave;
     const int hk = h / (p.H / p.HK);
     const uint16_t* kp = (const uint16_t*)p.k + b * p.k_sb + hk * p.k_sh;
     const uint16_t* vp = (const uint16_t*)p.v + b * p.v_sb + hk * p.v_sh;
-    const uint8_t* mask = p.mask ? p.mask + b * p.mask_sb : nullptr;
-    const int i = i0 + lane % 32, ic = min(i, p.S - 1);
+    const int i = i0 + lane % 32;
+    const int64_t ic = min(i, p.S - 1);
     Frag<T> q[D / 16], g[D / 16];
     float dl = 0.0f;
     {
@@ -318,48 +357,48 @@ __global__ __launch_bounds__(NT, 2) void k_attn_dq(D8sAttnArgs p, float* delta) 
     if (lane < 32 && i < p.S) delta[stat] = dl;
     const float c = p.scale * LOG2E, lse2 = lse2_of(p.lse[stat]);
     f32x16 acc[ND] = {};
-    const Tiles tiles = tiles_of<TILE>(p, i00, min(i00 + 127, p.S - 1));
-    Stage<D, TILE> sk, sv;
+    const Tiles tiles = tiles_of(p, i00, min(i00 + 127, p.S - 1));
+    const Copy<D, TILE> copy;
+    KeyBits keys{p.mask ? p.mask + b * p.mask_sb : nullptr, p.S, 1};
     int k0 = tiles.at(0) * TILE;
-    uint64_t bits = key_bits(mask, p.S, k0, lane);
-    sk.load(kp, p.k_ss, k0, p.S - 1);
-    sv.load(vp, p.v_ss, k0, p.S - 1);
-    sk.store(lk[0], bits);
-    sv.store(lv[0], bits);
-    __syncthreads();
+    copy(kp, p.k_ss, k0, p.S - 1, lk[0], wave);
+    copy(vp, p.v_ss, k0, p.S - 1, lv[0], wave);
+    keys.load(k0, lane);
     for (int t = 0; t < tiles.count; ++t) {
-        uint64_t next = 0;
-        int k1 = 0;
-        if (t + 1 < tiles.count) {
-            k1 = tiles.at(t + 1) * TILE;
-            next = key_bits(mask, p.S, k1, lane);
-            sk.load(kp, p.k_ss, k1, p.S - 1);
-            sv.load(vp, p.v_ss, k1, p.S - 1);
+        u32x4 *tk = lk[t & 1], *tv = lv[t & 1];
+        arrived();
+        const uint64_t bits = keys.bits(k0);
+        if (bits != ~0ull) {
+            copy.clear(tk, bits);
+            copy.clear(tv, bits);
         }
+        __syncthreads();
+        const int now = k0;
+        if (t + 1 < tiles.count) {
+            k0 = tiles.at(t + 1) * TILE;
+            copy(kp, p.k_ss, k0, p.S - 1, lk[(t + 1) & 1], wave);
+            copy(vp, p.v_ss, k0, p.S - 1, lv[(t + 1) & 1], wave);
+            keys.load(k0, lane);
+        }
+        if (bits == 0 || none_seen(p, i0, now, now + TILE - 1)) continue;
+        const bool part = bits != ~0ull || !all_seen(p, i0, now, now + TILE - 1);
+        const uint64_t vis = bits & bits_below(i + p.right + 1 - now) & (bits_from(i - p.left - now) | bits_below(p.sinks - now));
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int ku = k0 + 32 * u;
-            const uint32_t bu = (uint32_t)(bits >> (32 * u));
-            if (bu == 0 || none_seen(p, i0, ku, ku + 31)) continue;
-            const u32x4 *tk = lk[t & 1], *tv = lv[t & 1];
-            f32x16 s = {}, dp = {};
+            f32x16 s = mfma(rows_frag<T, D>(tk, 32 * u, 0, lane), q[0], f32x16{});
+            f32x16 dp = mfma(rows_frag<T, D>(tv, 32 * u, 0, lane), g[0], f32x16{});
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
+            for (int k = 1; k < D / 16; ++k) {
                 s = mfma(rows_frag<T, D>(tk, 32 * u, k, lane), q[k], s);
                 dp = mfma(rows_frag<T, D>(tv, 32 * u, k, lane), g[k], dp);
             }
-            const bool part = bu != ~0u || !all_seen(p, i0, ku, ku + 31);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = exp2_(__builtin_fmaf(s[r], c, -lse2));
+            for (int r = 0; r < 16; ++r) s[r] = exp2_(__builtin_fmaf(s[r], c, -lse2)) * (dp[r] - dl);
             if (part) {
+                const uint32_t mine = lane_rows((uint32_t)(vis >> (32 * u)), lane);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int j = row_of(r, lane);
-                    s[r] = (bu >> j & 1) && seen(p, i, ku + j) ? s[r] : 0.0f;
-                }
+                for (int r = 0; r < 16; ++r) s[r] = __uint_as_float(__float_as_uint(s[r]) & keep_mask(mine, r));
             }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] *= dp[r] - dl;
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 const Frag<T> ds = round_frag<T>(s, w);
@@ -368,25 +407,8 @@ __global__ __launch_bounds__(NT, 2) void k_attn_dq(D8sAttnArgs p, float* delta) 
                     acc[d] = mfma(cols_frag<T, D>(tk, 32 * u + 16 * w, 32 * d, lane), ds, acc[d]);
             }
         }
-        if (t + 1 < tiles.count) {
-            sk.store(lk[(t + 1) & 1], next);
-            sv.store(lv[(t + 1) & 1], next);
-        }
-        bits = next;
-        k0 = k1;
-        __syncthreads();
     }
-    if (i >= p.S) return;
-    T* o = (T*)p.dq + (((int64_t)b * p.S + i) * p.H + h) * D + 4 * (lane / 32);
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            float f[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) f[j] = acc[d][4 * w + j] * p.scale;
-            store_n<T, 4>(o + 32 * d + 8 * w, 4, f);
-        }
+    store_rows<T, ND>((T*)p.dq + (((int64_t)b * p.S + i) * p.H + h) * D, acc, p.scale, i < p.S, lane);
 }
 
 // ---- backward: keys and values ----------------------------------------------------------------------
@@ -400,20 +422,21 @@ struct KeySplit {
 
 template <class T, int D>
 __global__ __launch_bounds__(NT, 2) void k_attn_dkv(D8sAttnArgs p, const float* delta, float* part, KeySplit ks) {
-    constexpr int KEYS = 128, TILE = 64, ND = D / 32;
+    constexpr int KEYS = 128, ND = D / 32;
     __shared__ u32x4 lq[2][TILE * D / 8], lg[2][TILE * D / 8];
     __shared__ float ls[2][TILE], ld[2][TILE];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int nk = (p.S + KEYS - 1) / KEYS, G = p.H / p.HK;
     const int items = ks.sink_tiles * ks.sink_split + (nk - ks.sink_tiles) * ks.split;
     const int id = xcd_order(blockIdx.x, gridDim.x), item = id % items, bh = id / items, b = bh / p.HK, hk = bh % p.HK;
     const bool sink = item < ks.sink_tiles * ks.sink_split;
     const int rest = sink ? item : item - ks.sink_tiles * ks.sink_split, n = sink ? ks.sink_split : ks.split;
     const int kt = (sink ? 0 : ks.sink_tiles) + rest / n, cut = rest % n;
-    const int j0 = kt * KEYS, jw = j0 + 32 * wave, j = jw + lane % 32, jc = min(j, p.S - 1);
+    const int j0 = kt * KEYS, jw = j0 + 32 * wave, j = jw + lane % 32;
+    const int64_t jc = min(j, p.S - 1);
     const uint8_t* mask = p.mask ? p.mask + b * p.mask_sb : nullptr;
     const bool on = j < p.S && (mask == nullptr || mask[jc] != 0);
-    const uint64_t any = __ballot(on);
+    const bool any = __any(on);
     Frag<T> k[D / 16], v[D / 16];
     {
         const uint16_t* kp = (const uint16_t*)p.k + b * p.k_sb + hk * p.k_sh + jc * p.k_ss + 8 * (lane / 32);
@@ -425,66 +448,75 @@ __global__ __launch_bounds__(NT, 2) void k_attn_dkv(D8sAttnArgs p, const float* 
         }
     }
     // queries that see any of the keys: j0 - right .. j0 + 127 + left, to the end for a first token
-    const int lo = (int)max((int64_t)0, (int64_t)j0 - p.right) / TILE;
-    const int hi = j0 < p.sinks ? (p.S - 1) / TILE : (int)(min((int64_t)p.S - 1, (int64_t)j0 + KEYS - 1 + p.left) / TILE);
+    const int lo = max(0, j0 - p.right) / TILE;
+    const int hi = (j0 < p.sinks ? p.S - 1 : min(p.S - 1, j0 + KEYS - 1 + p.left)) / TILE;
     const int per = hi - lo + 1;
     const int t0 = (int)((int64_t)G * per * cut / n), t1 = (int)((int64_t)G * per * (cut + 1) / n);
     const float c = p.scale * LOG2E;
     f32x16 dk[ND] = {}, dv[ND] = {};
-    Stage<D, TILE> sq, sg;
+    const Copy<D, TILE> copy;
     float se = 0.0f, sd = 0.0f;
-    const auto load = [&](int t) __attribute__((always_inline)) {
-        const int h = hk * G + t / per, q0 = (lo + t % per) * TILE;
-        sq.load((const uint16_t*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, q0, p.S - 1);
-        sg.load((const uint16_t*)p.dout + b * p.do_sb + h * p.do_sh, p.do_ss, q0, p.S - 1);
+    int h = hk * G + t0 / per, qt = lo + t0 % per;         // of the tile whose copies are on their way
+    const auto load = [&](int buf) __attribute__((always_inline)) {
+        copy((const uint16_t*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, qt * TILE, p.S - 1, lq[buf], wave);
+        copy((const uint16_t*)p.dout + b * p.do_sb + h * p.do_sh, p.do_ss, qt * TILE, p.S - 1, lg[buf], wave);
         if (threadIdx.x < TILE) {
-            const int i = q0 + threadIdx.x;
+            const int i = qt * TILE + threadIdx.x;
             const int64_t at = ((int64_t)b * p.H + h) * p.S + min(i, p.S - 1);
-            se = i < p.S ? lse2_of(p.lse[at]) : INFINITY;
-            sd = i < p.S ? delta[at] : 0.0f;
+            se = i < p.S ? lse2_of(p.lse[at]) : INFINITY;  // (a row past the end: every P is 0)
+            sd = delta[at];
         }
     };
-    const auto store = [&](int t, int buf) __attribute__((always_inline)) {
-        const int left = p.S - (lo + t % per) * TILE;
-        const uint64_t rows = left >= 64 ? ~0ull : (1ull << left) - 1;
-        sq.store(lq[buf], rows);
-        sg.store(lg[buf], rows);
+    if (t0 < t1) load(0);
+    for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1, qn = qt * TILE;
+        arrived();
         if (threadIdx.x < TILE) {
             ls[buf][threadIdx.x] = se;
             ld[buf][threadIdx.x] = sd;
         }
-    };
-    if (t0 < t1) {
-        load(t0);
-        store(t0, 0);
-    }
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1;
-        if (t + 1 < t1) load(t + 1);
+        __syncthreads();                       // the tile is there, and the other one is no longer read
+        if (t + 1 < t1) {
+            if (++qt > hi) {
+                qt = lo;
+                ++h;
+            }
+            load(buf ^ 1);
+        }
+        if (!any) continue;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int q0 = (lo + t % per) * TILE + 32 * u;
-            if (any == 0 || q0 >= p.S || none_seen(p, q0, jw, jw + 31)) continue;
-            f32x16 s = {}, dp = {};
+            const int q0 = qn + 32 * u;
+            if (q0 >= p.S || none_seen(p, q0, jw, jw + 31)) continue;
+            f32x16 s = mfma(rows_frag<T, D>(lq[buf], 32 * u, 0, lane), k[0], f32x16{});
+            f32x16 dp = mfma(rows_frag<T, D>(lg[buf], 32 * u, 0, lane), v[0], f32x16{});
 #pragma unroll
-            for (int x = 0; x < D / 16; ++x) {
+            for (int x = 1; x < D / 16; ++x) {
                 s = mfma(rows_frag<T, D>(lq[buf], 32 * u, x, lane), k[x], s);
                 dp = mfma(rows_frag<T, D>(lg[buf], 32 * u, x, lane), v[x], dp);
             }
-            const bool cutoff = !all_seen(p, q0, jw, jw + 31);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const f32x4 e = *(const f32x4*)&ls[buf][32 * u + 8 * g + 4 * (lane / 32)];
                 const f32x4 d = *(const f32x4*)&ld[buf][32 * u + 8 * g + 4 * (lane / 32)];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    float w = exp2_(__builtin_fmaf(s[4 * g + r], c, -e[r]));
-                    if (cutoff) w = seen(p, q0 + row_of(4 * g + r, lane), j) ? w : 0.0f;
-                    s[4 * g + r] = w;
-                    dp[4 * g + r] = w * (dp[4 * g + r] - d[r]);
+                    s[4 * g + r] = exp2_(__builtin_fmaf(s[4 * g + r], c, -e[r]));
+                    dp[4 * g + r] = s[4 * g + r] * (dp[4 * g + r] - d[r]);
                 }
             }
+            if (!all_seen(p, q0, jw, jw + 31)) {
+                // query q0 + r sees key j: r >= j - right - q0, and r <= j + left - q0 or j is a first token
+                const uint64_t vis = bits_from(j - p.right - q0) & (j < p.sinks ? ~0ull : bits_below(j + p.left + 1 - q0));
+                const uint32_t mine = lane_rows((uint32_t)vis, lane);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const uint32_t keep = keep_mask(mine, r);
+                    s[r] = __uint_as_float(__float_as_uint(s[r]) & keep);
+                    dp[r] = __uint_as_float(__float_as_uint(dp[r]) & keep);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 const Frag<T> pf = round_frag<T>(s, w), df = round_frag<T>(dp, w);
@@ -494,12 +526,15 @@ __global__ __launch_bounds__(NT, 2) void k_attn_dkv(D8sAttnArgs p, const float* 
                     dk[d] = mfma(cols_frag<T, D>(lq[buf], 32 * u + 16 * w, 32 * d, lane), df, dk[d]);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (t + 1 < t1) store(t + 1, buf ^ 1);
-        __syncthreads();
     }
-    if (j >= p.S) return;
+    if (!on) {                                 // a masked key's column may hold anything: it has no gradient
+#pragma unroll
+        for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
+    }
     if (n > 1) {                               // part[problem and item][dk, dv][key][D]
+        if (j >= p.S) return;
         float* o = part + (int64_t)id * 2 * KEYS * D + (int64_t)(j - j0) * D + 4 * (lane / 32);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
@@ -508,28 +543,17 @@ __global__ __launch_bounds__(NT, 2) void k_attn_dkv(D8sAttnArgs p, const float* 
                 f32x4 x, y;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    x[r] = on ? dk[d][4 * g + r] * p.scale : 0.0f;
-                    y[r] = on ? dv[d][4 * g + r] : 0.0f;
+                    x[r] = dk[d][4 * g + r] * p.scale;
+                    y[r] = dv[d][4 * g + r];
                 }
                 *(f32x4*)(o + 32 * d + 8 * g) = x;
                 *(f32x4*)(o + KEYS * D + 32 * d + 8 * g) = y;
             }
         return;
     }
-    const int64_t at = (((int64_t)b * p.S + j) * p.HK + hk) * D + 4 * (lane / 32);
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            float x[4], y[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                x[r] = on ? dk[d][4 * g + r] * p.scale : 0.0f;
-                y[r] = on ? dv[d][4 * g + r] : 0.0f;
-            }
-            store_n<T, 4>((T*)p.dk + at + 32 * d + 8 * g, 4, x);
-            store_n<T, 4>((T*)p.dv + at + 32 * d + 8 * g, 4, y);
-        }
+    const int64_t at = (((int64_t)b * p.S + j) * p.HK + hk) * D;
+    store_rows<T, ND>((T*)p.dk + at, dk, p.scale, j < p.S, lane);
+    store_rows<T, ND>((T*)p.dv + at, dv, 1.0f, j < p.S, lane);
 }
 
 // dk and dv of the split tiles: the float32 parts summed in order, four values a thread
@@ -732,6 +756,15 @@ void token_run(const D8sTokenArgs& a, hipStream_t st) {
         hipLaunchKernelGGL((k_join<T, D>), dim3((unsigned)(a.B * a.H)), dim3(D), 0, st, part, (T*)a.out, split, a.B * a.H);
 }
 
+// The arguments with a window no wider than the tokens (the kernels add its sides to positions)
+D8sAttnArgs clipped(const D8sAttnArgs* a) {
+    D8sAttnArgs c = *a;
+    c.left = std::min(a->left, a->S);
+    c.right = std::min(a->right, a->S);
+    c.sinks = std::min(a->sinks, a->S);
+    return c;
+}
+
 template <class T, int D>
 void attn_run(const D8sAttnArgs& a, hipStream_t st) {
     const unsigned grid = (unsigned)((int64_t)a.B * a.H * ((a.S + 127) / 128));
@@ -763,7 +796,7 @@ int attn_check(const D8sAttnArgs* a, const char* what) {
     AREQ(a->dtype == D8S_BF16 || a->dtype == D8S_F16, "dtype must be D8S_BF16 or D8S_F16");
     AREQ(a->D == 64 || a->D == 128, "D must be 64 or 128");
     AREQ(a->B >= 1 && a->S >= 1 && a->H >= 1 && a->HK >= 1 && a->H % a->HK == 0, "bad sizes (H a multiple of HK)");
-    AREQ(a->S <= (1 << 30), "more than 2^30 tokens");
+    AREQ(a->S <= (1 << 29), "more than 2^29 tokens");
     AREQ((int64_t)a->B * a->H * ((a->S + 127) / 128) < (1 << 24), "too many heads and tokens");
     AREQ(a->left >= 0 && a->right >= 0 && a->sinks >= 0, "left, right and sinks must not be negative");
     AREQ(a->scale > 0 && a->scale < INFINITY, "scale must be positive and finite");
@@ -776,7 +809,7 @@ int attn_check(const D8sAttnArgs* a, const char* what) {
 extern "C" int d8s_attention(const D8sAttnArgs* a, void* stream) {
     const char* what = "d8s_attention";
     if (int rc = attn_check(a, what)) return rc;
-    BY_TYPE(attn_run, *a, (hipStream_t)stream);
+    BY_TYPE(attn_run, clipped(a), (hipStream_t)stream);
     return d8s_host_launched(what);
 }
 
@@ -799,7 +832,7 @@ extern "C" int d8s_attention_backward(const D8sAttnArgs* a, void* stream) {
     AREQ(a->ws_bytes >= need && ((uintptr_t)a->workspace & 15) == 0,
          "workspace smaller than d8s_attention_workspace() or not 16-byte aligned");
     AREQ((int64_t)a->B * a->HK * key_items(a, key_split(a)) < (1 << 24), "too many heads and tokens");
-    BY_TYPE(attn_back_run, *a, (hipStream_t)stream);
+    BY_TYPE(attn_back_run, clipped(a), (hipStream_t)stream);
     return d8s_host_launched(what);
 }
 
