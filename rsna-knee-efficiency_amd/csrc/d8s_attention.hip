@@ -51,34 +51,54 @@ DEV f32x16 mfma(Frag<f16> a, Frag<f16> b, f32x16 c) { return __builtin_amdgcn_mf
 
 DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// 16-byte pieces of a row of D values, and where piece c of row r lies
+// Where piece c (16 bytes) of row r of a tile lies: c ^ swizzle<D>(r).  The swizzle repeats every 16 rows.
 template <int D>
-DEV int piece(int r, int c) {
-    static_assert(D == 64 || D == 128, "row of 8 or 16 pieces");
+DEV int swizzle(int r) {
+    static_assert(D == 64 || D == 128, "rows of 8 or 16 pieces");
     if constexpr (D == 64) {
-        const int k = (r >> 1) & 7;            // rows r and r + 1 fill the banks once: the swizzle goes by pairs
-        return r * 8 + (c ^ ((k & 1) << 2 | (k & 2) | k >> 2));
+        const int k = (r >> 1) & 7;            // two rows fill the banks once: it goes by pairs
+        return (k & 1) << 2 | (k & 2) | k >> 2;
     } else {
-        return r * 16 + (c ^ ((r & 3) << 2 | (r >> 2 & 3)));
+        return (r & 3) << 2 | (r >> 2 & 3);
     }
 }
 
-// Operand of rows r0 .. r0 + 31, values 16 k .. 16 k + 15 of each
-template <class T, int D>
-DEV Frag<T> rows_frag(const u32x4* tile, int r0, int k, int lane) {
-    const u32x4 v = tile[piece<D>(r0 + lane % 32, 2 * k + lane / 32)];
-    return __builtin_bit_cast(Frag<T>, v);
+// LDS by byte address: every address of a tile's operands is the lane's first one with some bits flipped (the piece)
+// and a constant added (the rows), so two registers serve all of them.
+typedef __attribute__((address_space(3))) char* lds_bytes;
+DEV uint32_t lds_at(const void* p) { return (uint32_t)(uintptr_t)(lds_bytes)p; }
+
+// The lane's first address for rows_frag, and for cols_frag, relative to a tile
+template <int D>
+DEV uint32_t rows_at(int lane) {
+    const int r = lane % 32;
+    return r * 2 * D + ((lane / 32 ^ swizzle<D>(r)) << 4);
+}
+template <int D>
+DEV uint32_t cols_at(int lane) {
+    const int i = lane % 16, r = 4 * (lane / 32) + i / 4, c = 2 * (lane / 16 & 1) + (i % 4) / 2;
+    return r * 2 * D + ((c ^ swizzle<D>(r)) << 4) + 8 * (i & 1);
+}
+// Keeps the addresses derived from this one from being formed ahead of the loop and held in registers
+DEV uint32_t fresh(uint32_t at) {
+    asm volatile("" : "+v"(at));
+    return at;
 }
 
-// Operand of columns d0 .. d0 + 31, summed over the tile's rows r0 .. r0 + 15 in the order of a result's registers
+// Operand of rows r0 .. r0 + 31 (r0 a multiple of 16), values 16 k .. 16 k + 15 of each
 template <class T, int D>
-DEV Frag<T> cols_frag(const u32x4* tile, int r0, int d0, int lane) {
+DEV Frag<T> rows_frag(uint32_t at, int r0, int k) {
+    typedef const __attribute__((address_space(3))) u32x4* lds;
+    return __builtin_bit_cast(Frag<T>, *(lds)(uintptr_t)((at ^ (uint32_t)(k << 5)) + r0 * 2 * D));
+}
+
+// Operand of columns 32 d .. 32 d + 31, summed over the tile's rows r0 .. r0 + 15 in the order of a result's registers
+template <class T, int D>
+DEV Frag<T> cols_frag(uint32_t at, int r0, int d) {
     typedef __attribute__((address_space(3))) s16x4* lds;
-    const int i = lane % 16, r = r0 + 4 * (lane / 32) + i / 4;
-    const int c = d0 / 8 + 2 * (lane / 16 & 1) + (i % 4) / 2;
-    const char* lo = (const char*)(tile + piece<D>(r, c)) + 8 * (i & 1);
-    const char* hi = (const char*)(tile + piece<D>(r + 8, c)) + 8 * (i & 1);
-    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)lo), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)hi);
+    const uint32_t lo = at ^ (uint32_t)(d << 6), hi = lo ^ (D == 64 ? 16u : 32u);    // (8 rows on, the swizzle differs in one bit)
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(uintptr_t)(lo + r0 * 2 * D));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(uintptr_t)(hi + (r0 + 8) * 2 * D));
     typedef short s16x8 __attribute__((ext_vector_type(8)));
     const s16x8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(Frag<T>, v);
@@ -138,8 +158,8 @@ struct Copy {
     int row, col;                              // of the thread's first piece
     DEV Copy() {
         row = threadIdx.x / P;
-        col = 8 * (piece<D>(row, threadIdx.x % P) % P);    // (the swizzle is its own inverse, and repeats every STEP rows)
-        static_assert(STEP % 16 == 0, "swizzle");
+        col = 8 * (threadIdx.x % P ^ swizzle<D>(row));
+        static_assert(STEP % 16 == 0, "the same swizzle for all of a thread's pieces");
     }
     DEV void operator()(const uint16_t* p, int64_t stride, int r0, int last, u32x4* tile, int wave) const {
         typedef const __attribute__((address_space(1))) void* global;
@@ -256,12 +276,13 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
             keys.load(k0, lane);
         }
         if (bits == 0 || none_seen(p, i0, now, now + TILE - 1)) continue;
+        const uint32_t rk = fresh(lds_at(tk) + rows_at<D>(lane)), cv = fresh(lds_at(tv) + cols_at<D>(lane));
         f32x16 s[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            s[u] = mfma(rows_frag<T, D>(tk, 32 * u, 0, lane), q[0], f32x16{});
+            s[u] = mfma(rows_frag<T, D>(rk, 32 * u, 0), q[0], f32x16{});
 #pragma unroll
-            for (int k = 1; k < D / 16; ++k) s[u] = mfma(rows_frag<T, D>(tk, 32 * u, k, lane), q[k], s[u]);
+            for (int k = 1; k < D / 16; ++k) s[u] = mfma(rows_frag<T, D>(rk, 32 * u, k), q[k], s[u]);
         }
         if (bits != ~0ull || !all_seen(p, i0, now, now + TILE - 1)) {
             const uint64_t vis = bits & bits_below(i + p.right + 1 - now) & (bits_from(i - p.left - now) | bits_below(p.sinks - now));
@@ -306,7 +327,7 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
         for (int u = 0; u < 4; ++u) {
             const Frag<T> w = round_frag<T>(s[u / 2], u % 2);
 #pragma unroll
-            for (int d = 0; d < ND; ++d) acc[d] = mfma(cols_frag<T, D>(tv, 16 * u, 32 * d, lane), w, acc[d]);
+            for (int d = 0; d < ND; ++d) acc[d] = mfma(cols_frag<T, D>(cv, 16 * u, d), w, acc[d]);
         }
     }
     float l0, l1;
@@ -381,16 +402,18 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn_dq(D8sAttnArgs p
             keys.load(k0, lane);
         }
         if (bits == 0 || none_seen(p, i0, now, now + TILE - 1)) continue;
+        const uint32_t rk = fresh(lds_at(tk) + rows_at<D>(lane)), rv = fresh(lds_at(tv) + rows_at<D>(lane));
+        const uint32_t ck = fresh(lds_at(tk) + cols_at<D>(lane));
         const bool part = bits != ~0ull || !all_seen(p, i0, now, now + TILE - 1);
         const uint64_t vis = bits & bits_below(i + p.right + 1 - now) & (bits_from(i - p.left - now) | bits_below(p.sinks - now));
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            f32x16 s = mfma(rows_frag<T, D>(tk, 32 * u, 0, lane), q[0], f32x16{});
-            f32x16 dp = mfma(rows_frag<T, D>(tv, 32 * u, 0, lane), g[0], f32x16{});
+            f32x16 s = mfma(rows_frag<T, D>(rk, 32 * u, 0), q[0], f32x16{});
+            f32x16 dp = mfma(rows_frag<T, D>(rv, 32 * u, 0), g[0], f32x16{});
 #pragma unroll
             for (int k = 1; k < D / 16; ++k) {
-                s = mfma(rows_frag<T, D>(tk, 32 * u, k, lane), q[k], s);
-                dp = mfma(rows_frag<T, D>(tv, 32 * u, k, lane), g[k], dp);
+                s = mfma(rows_frag<T, D>(rk, 32 * u, k), q[k], s);
+                dp = mfma(rows_frag<T, D>(rv, 32 * u, k), g[k], dp);
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = exp2_(__builtin_fmaf(s[r], c, -lse2)) * (dp[r] - dl);
@@ -404,7 +427,7 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn_dq(D8sAttnArgs p
                 const Frag<T> ds = round_frag<T>(s, w);
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
-                    acc[d] = mfma(cols_frag<T, D>(tk, 32 * u + 16 * w, 32 * d, lane), ds, acc[d]);
+                    acc[d] = mfma(cols_frag<T, D>(ck, 32 * u + 16 * w, d), ds, acc[d]);
             }
         }
     }
@@ -412,48 +435,56 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn_dq(D8sAttnArgs p
 }
 
 // ---- backward: keys and values ----------------------------------------------------------------------
-// A workgroup runs 128 keys of a key head, 32 a wave, over the tiles of 64 queries that see them, one query head of
-// the group after the other, so that dk and dv of shared heads are sums within one workgroup, in a fixed order.  The
+// A workgroup runs 128 KB keys of a key head, 32 KB a wave, over the tiles of 64 queries that see them, one query head
+// of the group after the other, so that dk and dv of shared heads are sums within one workgroup, in a fixed order.  The
 // tiles of the first tokens are seen by every query: their queries are split over `sink_split` workgroups (and all
 // tiles' over `split` where there are fewer tiles than compute units), whose float32 sums k_attn_join adds.
+// The products start from -lse / scale and -rowsum(do o) in place of zero, so P and dS are an exponential and a product.
 struct KeySplit {
     int sink_tiles, sink_split, split;
 };
+template <int D>
+constexpr int KB = 1;                          // blocks of 32 keys a wave
+template <int D>
+constexpr int KEYS = 128 * KB<D>;
 
 template <class T, int D>
 __global__ __launch_bounds__(NT, 2) void k_attn_dkv(D8sAttnArgs p, const float* delta, float* part, KeySplit ks) {
-    constexpr int KEYS = 128, ND = D / 32;
+    constexpr int ND = D / 32, NB = KB<D>;
     __shared__ u32x4 lq[2][TILE * D / 8], lg[2][TILE * D / 8];
     __shared__ float ls[2][TILE], ld[2][TILE];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int nk = (p.S + KEYS - 1) / KEYS, G = p.H / p.HK;
+    const int nk = (p.S + KEYS<D> - 1) / KEYS<D>, G = p.H / p.HK;
     const int items = ks.sink_tiles * ks.sink_split + (nk - ks.sink_tiles) * ks.split;
     const int id = xcd_order(blockIdx.x, gridDim.x), item = id % items, bh = id / items, b = bh / p.HK, hk = bh % p.HK;
     const bool sink = item < ks.sink_tiles * ks.sink_split;
     const int rest = sink ? item : item - ks.sink_tiles * ks.sink_split, n = sink ? ks.sink_split : ks.split;
     const int kt = (sink ? 0 : ks.sink_tiles) + rest / n, cut = rest % n;
-    const int j0 = kt * KEYS, jw = j0 + 32 * wave, j = jw + lane % 32;
-    const int64_t jc = min(j, p.S - 1);
+    const int j0 = kt * KEYS<D>, jw = j0 + 32 * NB * wave, jl = jw + lane % 32;
     const uint8_t* mask = p.mask ? p.mask + b * p.mask_sb : nullptr;
-    const bool on = j < p.S && (mask == nullptr || mask[jc] != 0);
-    const bool any = __any(on);
-    Frag<T> k[D / 16], v[D / 16];
-    {
+    bool on[NB], any = false;
+    Frag<T> k[NB][D / 16], v[NB][D / 16];
+#pragma unroll
+    for (int y = 0; y < NB; ++y) {
+        const int64_t jc = min(jl + 32 * y, p.S - 1);
+        on[y] = jl + 32 * y < p.S && (mask == nullptr || mask[jc] != 0);
+        any |= on[y];
         const uint16_t* kp = (const uint16_t*)p.k + b * p.k_sb + hk * p.k_sh + jc * p.k_ss + 8 * (lane / 32);
         const uint16_t* vp = (const uint16_t*)p.v + b * p.v_sb + hk * p.v_sh + jc * p.v_ss + 8 * (lane / 32);
 #pragma unroll
         for (int u = 0; u < D / 16; ++u) {
-            k[u] = __builtin_bit_cast(Frag<T>, *(const Raw*)(kp + 16 * u));
-            v[u] = __builtin_bit_cast(Frag<T>, *(const Raw*)(vp + 16 * u));
+            k[y][u] = __builtin_bit_cast(Frag<T>, *(const Raw*)(kp + 16 * u));
+            v[y][u] = __builtin_bit_cast(Frag<T>, *(const Raw*)(vp + 16 * u));
         }
     }
-    // queries that see any of the keys: j0 - right .. j0 + 127 + left, to the end for a first token
+    any = __any(any);
+    // queries that see any of the keys: from j0 - right, to left past the last key or the end for a first token
     const int lo = max(0, j0 - p.right) / TILE;
-    const int hi = (j0 < p.sinks ? p.S - 1 : min(p.S - 1, j0 + KEYS - 1 + p.left)) / TILE;
+    const int hi = (j0 < p.sinks ? p.S - 1 : min(p.S - 1, j0 + KEYS<D> - 1 + p.left)) / TILE;
     const int per = hi - lo + 1;
     const int t0 = (int)((int64_t)G * per * cut / n), t1 = (int)((int64_t)G * per * (cut + 1) / n);
-    const float c = p.scale * LOG2E;
-    f32x16 dk[ND] = {}, dv[ND] = {};
+    const float c = p.scale * LOG2E, c1 = 1.0f / p.scale;
+    f32x16 dk[NB][ND] = {}, dv[NB][ND] = {};
     const Copy<D, TILE> copy;
     float se = 0.0f, sd = 0.0f;
     int h = hk * G + t0 / per, qt = lo + t0 % per;         // of the tile whose copies are on their way
@@ -463,8 +494,9 @@ __global__ __launch_bounds__(NT, 2) void k_attn_dkv(D8sAttnArgs p, const float* 
         if (threadIdx.x < TILE) {
             const int i = qt * TILE + threadIdx.x;
             const int64_t at = ((int64_t)b * p.H + h) * p.S + min(i, p.S - 1);
-            se = i < p.S ? lse2_of(p.lse[at]) : INFINITY;  // (a row past the end: every P is 0)
-            sd = delta[at];
+            const float e = p.lse[at];         // (a row past the end, or that sees nothing: every P is 0)
+            se = i < p.S && e != -INFINITY ? -e * c1 : -INFINITY;
+            sd = -delta[at];
         }
     };
     if (t0 < t1) load(0);
@@ -484,82 +516,112 @@ __global__ __launch_bounds__(NT, 2) void k_attn_dkv(D8sAttnArgs p, const float* 
             load(buf ^ 1);
         }
         if (!any) continue;
+        const uint32_t rq = fresh(lds_at(lq[buf]) + rows_at<D>(lane)), rg = fresh(lds_at(lg[buf]) + rows_at<D>(lane));
+        const uint32_t cq = fresh(lds_at(lq[buf]) + cols_at<D>(lane)), cg = fresh(lds_at(lg[buf]) + cols_at<D>(lane));
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int q0 = qn + 32 * u;
-            if (q0 >= p.S || none_seen(p, q0, jw, jw + 31)) continue;
-            f32x16 s = mfma(rows_frag<T, D>(lq[buf], 32 * u, 0, lane), k[0], f32x16{});
-            f32x16 dp = mfma(rows_frag<T, D>(lg[buf], 32 * u, 0, lane), v[0], f32x16{});
-#pragma unroll
-            for (int x = 1; x < D / 16; ++x) {
-                s = mfma(rows_frag<T, D>(lq[buf], 32 * u, x, lane), k[x], s);
-                dp = mfma(rows_frag<T, D>(lg[buf], 32 * u, x, lane), v[x], dp);
-            }
+            if (q0 >= p.S || none_seen(p, q0, jw, jw + 32 * NB - 1)) continue;
+            f32x16 s[NB], dp[NB];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const f32x4 e = *(const f32x4*)&ls[buf][32 * u + 8 * g + 4 * (lane / 32)];
                 const f32x4 d = *(const f32x4*)&ld[buf][32 * u + 8 * g + 4 * (lane / 32)];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s[4 * g + r] = exp2_(__builtin_fmaf(s[4 * g + r], c, -e[r]));
-                    dp[4 * g + r] = s[4 * g + r] * (dp[4 * g + r] - d[r]);
+                for (int y = 0; y < NB; ++y)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        s[y][4 * g + r] = e[r];
+                        dp[y][4 * g + r] = d[r];
+                    }
+            }
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x) {
+                const Frag<T> fq = rows_frag<T, D>(rq, 32 * u, x), fg = rows_frag<T, D>(rg, 32 * u, x);
+#pragma unroll
+                for (int y = 0; y < NB; ++y) {
+                    s[y] = mfma(fq, k[y][x], s[y]);
+                    dp[y] = mfma(fg, v[y][x], dp[y]);
                 }
             }
-            if (!all_seen(p, q0, jw, jw + 31)) {
-                // query q0 + r sees key j: r >= j - right - q0, and r <= j + left - q0 or j is a first token
-                const uint64_t vis = bits_from(j - p.right - q0) & (j < p.sinks ? ~0ull : bits_below(j + p.left + 1 - q0));
-                const uint32_t mine = lane_rows((uint32_t)vis, lane);
+#pragma unroll
+            for (int y = 0; y < NB; ++y)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const uint32_t keep = keep_mask(mine, r);
-                    s[r] = __uint_as_float(__float_as_uint(s[r]) & keep);
-                    dp[r] = __uint_as_float(__float_as_uint(dp[r]) & keep);
+                    s[y][r] = exp2_(s[y][r] * c);
+                    dp[y][r] *= s[y][r];
+                }
+            if (!all_seen(p, q0, jw, jw + 32 * NB - 1)) {
+#pragma unroll
+                for (int y = 0; y < NB; ++y) {
+                    // query q0 + r sees key j: r >= j - right - q0, and r <= j + left - q0 or j is a first token
+                    const int j = jl + 32 * y;
+                    const uint64_t vis = bits_from(j - p.right - q0) & (j < p.sinks ? ~0ull : bits_below(j + p.left + 1 - q0));
+                    const uint32_t mine = lane_rows((uint32_t)vis, lane);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const uint32_t keep = keep_mask(mine, r);
+                        s[y][r] = __uint_as_float(__float_as_uint(s[y][r]) & keep);
+                        dp[y][r] = __uint_as_float(__float_as_uint(dp[y][r]) & keep);
+                    }
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-                const Frag<T> pf = round_frag<T>(s, w), df = round_frag<T>(dp, w);
+                Frag<T> pf[NB], df[NB];
+#pragma unroll
+                for (int y = 0; y < NB; ++y) {
+                    pf[y] = round_frag<T>(s[y], w);
+                    df[y] = round_frag<T>(dp[y], w);
+                }
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    dv[d] = mfma(cols_frag<T, D>(lg[buf], 32 * u + 16 * w, 32 * d, lane), pf, dv[d]);
-                    dk[d] = mfma(cols_frag<T, D>(lq[buf], 32 * u + 16 * w, 32 * d, lane), df, dk[d]);
+                    const Frag<T> fg = cols_frag<T, D>(cg, 32 * u + 16 * w, d), fq = cols_frag<T, D>(cq, 32 * u + 16 * w, d);
+#pragma unroll
+                    for (int y = 0; y < NB; ++y) {
+                        dv[y][d] = mfma(fg, pf[y], dv[y][d]);
+                        dk[y][d] = mfma(fq, df[y], dk[y][d]);
+                    }
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
         }
     }
-    if (!on) {                                 // a masked key's column may hold anything: it has no gradient
 #pragma unroll
-        for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
-    }
-    if (n > 1) {                               // part[problem and item][dk, dv][key][D]
-        if (j >= p.S) return;
-        float* o = part + (int64_t)id * 2 * KEYS * D + (int64_t)(j - j0) * D + 4 * (lane / 32);
+    for (int y = 0; y < NB; ++y) {
+        const int j = jl + 32 * y;
+        if (!on[y]) {                          // a masked key's column may hold anything: it has no gradient
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
+            for (int d = 0; d < ND; ++d) dk[y][d] = dv[y][d] = f32x16{};
+        }
+        if (n > 1) {                           // part[problem and item][dk, dv][key][D]
+            float* o = part + (int64_t)id * 2 * KEYS<D> * D + (int64_t)(j - j0) * D + 4 * (lane / 32);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                f32x4 x, y;
+            for (int d = 0; d < ND; ++d)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    x[r] = dk[d][4 * g + r] * p.scale;
-                    y[r] = dv[d][4 * g + r];
+                for (int g = 0; g < 4; ++g) {
+                    f32x4 x, z;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        x[r] = dk[y][d][4 * g + r] * p.scale;
+                        z[r] = dv[y][d][4 * g + r];
+                    }
+                    if (j < p.S) {
+                        *(f32x4*)(o + 32 * d + 8 * g) = x;
+                        *(f32x4*)(o + KEYS<D> * D + 32 * d + 8 * g) = z;
+                    }
                 }
-                *(f32x4*)(o + 32 * d + 8 * g) = x;
-                *(f32x4*)(o + KEYS * D + 32 * d + 8 * g) = y;
-            }
-        return;
+        } else {
+            const int64_t at = (((int64_t)b * p.S + j) * p.HK + hk) * D;
+            store_rows<T, ND>((T*)p.dk + at, dk[y], p.scale, j < p.S, lane);
+            store_rows<T, ND>((T*)p.dv + at, dv[y], 1.0f, j < p.S, lane);
+        }
     }
-    const int64_t at = (((int64_t)b * p.S + j) * p.HK + hk) * D;
-    store_rows<T, ND>((T*)p.dk + at, dk, p.scale, j < p.S, lane);
-    store_rows<T, ND>((T*)p.dv + at, dv, 1.0f, j < p.S, lane);
 }
 
 // dk and dv of the split tiles: the float32 parts summed in order, four values a thread
 template <class T, int D>
 __global__ __launch_bounds__(NT) void k_attn_join(D8sAttnArgs p, const float* part, KeySplit ks) {
-    constexpr int KEYS = 128;
+    constexpr int KEYS = 128 * KB<D>;
     const int nk = (p.S + KEYS - 1) / KEYS, items = ks.sink_tiles * ks.sink_split + (nk - ks.sink_tiles) * ks.split;
     const int joined = ks.split > 1 ? nk : ks.sink_tiles;          // tiles per problem, the first ones
     const int kt = blockIdx.x % joined, bh = blockIdx.x / joined, b = bh / p.HK, hk = bh % p.HK;
@@ -578,17 +640,17 @@ __global__ __launch_bounds__(NT) void k_attn_join(D8sAttnArgs p, const float* pa
 }
 
 KeySplit key_split(const D8sAttnArgs* a) {
-    const int64_t S = a->S, nk = (S + 127) / 128, nq = (S + 63) / 64, G = a->H / a->HK;
-    const int64_t seen = std::min(nq, (std::min<int64_t>(a->left, S) + std::min<int64_t>(a->right, S) + 128) / 64 + 1);
+    const int64_t S = a->S, keys = a->D == 64 ? KEYS<64> : KEYS<128>, nk = (S + keys - 1) / keys, nq = (S + 63) / 64, G = a->H / a->HK;
+    const int64_t seen = std::min(nq, (std::min<int64_t>(a->left, S) + std::min<int64_t>(a->right, S) + keys) / 64 + 1);
     const int64_t cus = d8s_host_cu_count(), problems = (int64_t)a->B * a->HK;
     KeySplit k;
     k.split = (int)std::max<int64_t>(1, std::min(cus / std::max<int64_t>(1, problems * nk), G * seen / 4));
-    k.sink_tiles = (int)std::min(nk, ((int64_t)a->sinks + 127) / 128);
+    k.sink_tiles = (int)std::min(nk, ((int64_t)a->sinks + keys - 1) / keys);
     k.sink_split = (int)std::min<int64_t>(G * nq, (k.split * nq + seen - 1) / seen);
     return k;
 }
 int64_t key_items(const D8sAttnArgs* a, const KeySplit& k) {
-    const int64_t nk = (a->S + 127) / 128;
+    const int keys = a->D == 64 ? KEYS<64> : KEYS<128>, nk = (a->S + keys - 1) / keys;
     return (int64_t)k.sink_tiles * k.sink_split + (nk - k.sink_tiles) * k.split;
 }
 uint64_t delta_bytes(const D8sAttnArgs* a) { return ((uint64_t)a->B * a->H * a->S * 4 + 255) / 256 * 256; }
@@ -777,11 +839,11 @@ void attn_back_run(const D8sAttnArgs& a, hipStream_t st) {
     float* part = (float*)((char*)a.workspace + delta_bytes(&a));
     const KeySplit ks = key_split(&a);
     const unsigned grid = (unsigned)((int64_t)a.B * a.H * ((a.S + 127) / 128));
-    const int problems = a.B * a.HK, nk = (a.S + 127) / 128, joined = ks.split > 1 ? nk : ks.sink_split > 1 ? ks.sink_tiles : 0;
+    const int problems = a.B * a.HK, nk = (a.S + KEYS<D> - 1) / KEYS<D>, joined = ks.split > 1 ? nk : ks.sink_split > 1 ? ks.sink_tiles : 0;
     hipLaunchKernelGGL((k_attn_dq<T, D>), dim3(grid), dim3(NT), 0, st, a, delta);
     hipLaunchKernelGGL((k_attn_dkv<T, D>), dim3((unsigned)(problems * key_items(&a, ks))), dim3(NT), 0, st, a, delta, part, ks);
     if (joined)
-        hipLaunchKernelGGL((k_attn_join<T, D>), dim3((unsigned)(problems * joined), 2 * 128 * D / (4 * NT)), dim3(NT), 0, st,
+        hipLaunchKernelGGL((k_attn_join<T, D>), dim3((unsigned)(problems * joined), 2 * KEYS<D> * D / (4 * NT)), dim3(NT), 0, st,
                            a, part, ks);
 }
 
@@ -819,7 +881,7 @@ extern "C" int d8s_attention_workspace(const D8sAttnArgs* a, uint64_t* bytes) {
     AREQ(bytes != nullptr, "null arguments");
     const KeySplit k = key_split(a);
     const bool parts = k.split > 1 || (k.sink_tiles > 0 && k.sink_split > 1);
-    *bytes = delta_bytes(a) + (parts ? (uint64_t)a->B * a->HK * key_items(a, k) * 2 * 128 * a->D * 4 : 0);
+    *bytes = delta_bytes(a) + (parts ? (uint64_t)a->B * a->HK * key_items(a, k) * 2 * (a->D == 64 ? KEYS<64> : KEYS<128>) * a->D * 4 : 0);
     return 0;
 }
 
