@@ -10,7 +10,6 @@ into HIP graphs.  There is no CPU path: without the library the calls raise.
 """
 from __future__ import annotations
 
-import ctypes
 import functools
 import math
 
@@ -18,57 +17,37 @@ import torch
 
 from . import hip
 
-_byref, _vp = ctypes.byref, ctypes.c_void_p
-
-
 def _fail(message: str):
     raise ValueError(message)
 
 
-def _launch(name: str, args, device: torch.device) -> None:
-    """Calls entry point `name` on the current stream of `device`, with that device current."""
-    if torch.cuda.current_device() == device.index:
-        hip.call(name, _byref(args), _vp(torch.cuda.current_stream().cuda_stream))
-    else:
-        with torch.cuda.device(device):
-            hip.call(name, _byref(args), _vp(torch.cuda.current_stream().cuda_stream))
-
-
-def _bytes(name: str, args, device: torch.device) -> torch.Tensor:
-    """A work buffer of the size that `name` asks for (at least one byte), of this call alone."""
-    need = ctypes.c_uint64()
-    with torch.cuda.device(device):
-        hip.call(name, _byref(args), _byref(need))
-    return torch.empty(max(1, need.value), dtype=torch.uint8, device=device)
-
-
 def _on_gpu(*tensors: torch.Tensor) -> None:
     device = tensors[0].device
-    for t in tensors:
-        if t.device.type != "cuda" or t.device != device:
-            _fail("the tensors must be on one GPU")
+    if device.type != "cuda" or any(t.device != device for t in tensors):
+        _fail("the tensors must be on one GPU")
 
 
 # --- layer norm -----------------------------------------------------------------------------------
 NORM_MAX = 16384
 
 
-def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
+def _rows(x: torch.Tensor) -> torch.Tensor:
     """x as rows of its last dimension, evenly apart; copied only where its strides allow no such view"""
     x = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
-    return x if x.stride(1) == 1 and (x.stride(0) >= x.shape[1] or x.shape[0] == 1) else x.contiguous()
+    apart, step = x.stride()
+    return x if step == 1 and (apart >= x.shape[1] or x.shape[0] == 1) else x.contiguous()
 
 
-def _norm_args(x: torch.Tensor, weight: torch.Tensor) -> hip.NormArgs:
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= NORM_MAX:
+def _norm_types(x: torch.Tensor, weight: torch.Tensor) -> tuple[int, int, int]:
+    """(width, type of x, type of weight)"""
+    shape = x.shape
+    if not shape or not 1 <= shape[-1] <= NORM_MAX:
         _fail(f"x must have a last dimension of 1 .. {NORM_MAX}")
     if x.dtype not in hip.ELEMENTS:
         _fail("x must be float32, bfloat16 or float16")
-    if weight.shape != x.shape[-1:] or weight.dtype not in (torch.float32, x.dtype):
+    if weight.shape != shape[-1:] or weight.dtype not in (torch.float32, x.dtype):
         _fail("weight must have x's last dimension, in float32 or x's type")
-    a = hip.NormArgs()
-    a.width, a.dtype, a.wdtype = x.shape[-1], hip.ELEMENTS[x.dtype], hip.ELEMENTS[weight.dtype]
-    return a
+    return shape[-1], hip.ELEMENTS[x.dtype], hip.ELEMENTS[weight.dtype]
 
 
 def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, eps: float = 1e-5,
@@ -76,48 +55,49 @@ def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor
     """x (..., width) in float32, bfloat16 or float16; weight and bias (width,) in float32 or x's type ->
     (y like x, mean, rstd), the last two float32, one a row, for `layer_norm_backward` (None without
     `statistics`)."""
-    a = _norm_args(x, weight)
+    width, dtype, wdtype = _norm_types(x, weight)
     if bias is not None and (bias.shape != weight.shape or bias.dtype != weight.dtype):
         _fail("bias must be like weight")
-    _on_gpu(x, weight, *(() if bias is None else (bias,)))
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, x.numel() // x.shape[-1]), dtype=torch.float32, device=x.device) if statistics else (None, None)
-    if x.numel():
-        rows, weight = _rows(x, "x"), weight.contiguous()
+    device = x.device
+    _on_gpu(x, weight, weight if bias is None else bias)
+    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    n = x.numel() // width
+    mean = rstd = None
+    if statistics:
+        mean, rstd = (torch.empty(n, dtype=torch.float32, device=device) for _ in range(2))
+    if n:
+        rows, weight = _rows(x), weight.contiguous()
         bias = None if bias is None else bias.contiguous()
-        a.x, a.w, a.b, a.y = rows.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), y.data_ptr()
-        if statistics:
-            a.mean = stats.data_ptr()
-            a.rstd = a.mean + 4 * rows.shape[0]
-        a.rows, a.x_stride, a.eps = rows.shape[0], rows.stride(0), eps
-        _launch("d8s_layer_norm", a, x.device)
-    return y, stats[0], stats[1]
+        a = hip.NormArgs(rows.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), y.data_ptr(),
+                         mean.data_ptr() if statistics else 0, rstd.data_ptr() if statistics else 0, 0, 0, 0, 0, 0, 0,
+                         n, rows.stride(0), 0, width, dtype, wdtype, eps)
+        hip.launch("d8s_layer_norm", device, a)
+    return y, mean, rstd
 
 
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, mean: torch.Tensor,
                         rstd: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The gradients (dx like x, dweight, dbias like weight) of `layer_norm_forward` at dy like x."""
-    a = _norm_args(x, weight)
-    n = x.numel() // x.shape[-1]
+    width, dtype, wdtype = _norm_types(x, weight)
+    n = x.numel() // width
     if dy.shape != x.shape or dy.dtype != x.dtype:
         _fail("dy must be like x")
     if mean.shape != (n,) or rstd.shape != (n,) or mean.dtype != torch.float32 or rstd.dtype != torch.float32:
         _fail("mean and rstd must be float32, one a row")
+    device = x.device
     _on_gpu(x, dy, weight, mean, rstd)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=device)
     if not n:
         return dx, torch.zeros_like(weight), torch.zeros_like(weight)
-    dwb = torch.empty((2, x.shape[-1]), dtype=weight.dtype, device=x.device)
-    rows, grad, weight, mean, rstd = _rows(x, "x"), _rows(dy, "dy"), weight.contiguous(), mean.contiguous(), rstd.contiguous()
-    a.x, a.w, a.dy, a.dx = rows.data_ptr(), weight.data_ptr(), grad.data_ptr(), dx.data_ptr()
-    a.dw = dwb.data_ptr()
-    a.db = a.dw + dwb.element_size() * x.shape[-1]
-    a.mean, a.rstd = mean.data_ptr(), rstd.data_ptr()
-    a.rows, a.x_stride, a.dy_stride = n, rows.stride(0), grad.stride(0)
-    work = _bytes("d8s_layer_norm_workspace", a, x.device)
+    dw, db = (torch.empty(width, dtype=weight.dtype, device=device) for _ in range(2))
+    rows, grad, weight, mean, rstd = _rows(x), _rows(dy), weight.contiguous(), mean.contiguous(), rstd.contiguous()
+    a = hip.NormArgs(rows.data_ptr(), weight.data_ptr(), 0, 0, mean.data_ptr(), rstd.data_ptr(), grad.data_ptr(),
+                     dx.data_ptr(), dw.data_ptr(), db.data_ptr(), 0, 0, n, rows.stride(0), grad.stride(0), width, dtype,
+                     wdtype, 0.0)
+    work = hip.work_buffer("d8s_layer_norm_workspace", device, a)
     a.partial, a.partial_bytes = work.data_ptr(), work.numel()
-    _launch("d8s_layer_norm_backward", a, x.device)
-    return dx, dwb[0], dwb[1]
+    hip.launch("d8s_layer_norm_backward", device, a)
+    return dx, dw, db
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -187,7 +167,7 @@ def _rotate(x, positions, sections, base, adjacent, inverse, out):
     a.pos_sb = positions.stride(0) if positions.dim() == 3 else 0
     a.B, a.S, a.H, a.D = x.shape
     a.dtype, a.pos_type, a.adjacent, a.inverse = hip.ELEMENTS[x.dtype], _POSITIONS[positions.dtype], adjacent, inverse
-    _launch("d8s_rotary", a, x.device)
+    hip.launch("d8s_rotary", x.device, a)
     return out
 
 
@@ -241,7 +221,8 @@ def _extent(n: int | None, name: str) -> int:
 
 
 def _attn_args(q, k, v, left, right, sinks, key_mask, scale):
-    """The call's arguments, and the tensors they point into (a copy where the channels were not contiguous)"""
+    """The call's arguments, and the tensors they point into (copies where the channels were not contiguous), which the
+    caller holds until the call has been made"""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         _fail("q must be (batch, tokens, heads, channels), k and v (batch, tokens, key heads, channels)")
     B, S, H, D = q.shape
@@ -257,19 +238,16 @@ def _attn_args(q, k, v, left, right, sinks, key_mask, scale):
         _fail("scale must be positive and finite")
     q, k, v = _last(q), _last(k), _last(v)
     _on_gpu(q, k, v)
-    a = hip.AttnArgs()
+    mask_at, mask_sb = 0, 0
     if key_mask is not None:
         if key_mask.shape != (B, S) or key_mask.dtype not in (torch.bool, torch.uint8):
             _fail("key_mask must be (batch, tokens) of bool or uint8")
         _on_gpu(q, key_mask)
         key_mask = _last(key_mask)
-        a.mask, a.mask_sb = key_mask.data_ptr(), key_mask.stride(0)
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_sb, a.q_ss, a.q_sh = q.stride()[:3]
-    a.k_sb, a.k_ss, a.k_sh = k.stride()[:3]
-    a.v_sb, a.v_ss, a.v_sh = v.stride()[:3]
-    a.B, a.S, a.H, a.HK, a.D, a.dtype, a.scale = B, S, H, HK, D, hip.ELEMENTS[q.dtype], scale
-    a.left, a.right, a.sinks = _extent(left, "left"), _extent(right, "right"), _extent(sinks, "sinks")
+        mask_at, mask_sb = key_mask.data_ptr(), key_mask.stride(0)
+    a = hip.AttnArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), mask_at, 0, 0, 0, 0, 0, 0, 0, 0, *q.stride()[:3],
+                     *k.stride()[:3], *v.stride()[:3], 0, 0, 0, mask_sb, B, S, H, HK, D, hip.ELEMENTS[q.dtype],
+                     _extent(left, "left"), _extent(right, "right"), _extent(sinks, "sinks"), scale)
     return a, (q, k, v, key_mask)
 
 
@@ -285,13 +263,12 @@ def window_attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
 
     -> (out like q, lse (batch, heads, tokens) float32: the logarithm of the sum of exponentials, -inf where nothing
     is seen; None without `statistics`)"""
-    a, kept = _attn_args(q, k, v, left, right, sinks, key_mask, scale)
+    a, _kept = _attn_args(q, k, v, left, right, sinks, key_mask, scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((a.B, a.H, a.S), dtype=torch.float32, device=q.device) if statistics else None
     if q.numel():
         a.out, a.lse = out.data_ptr(), lse.data_ptr() if statistics else 0
-        _launch("d8s_attention", a, q.device)
-    del kept
+        hip.launch("d8s_attention", q.device, a)
     return out, lse
 
 
@@ -299,7 +276,7 @@ def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
                               lse: torch.Tensor, left: int | None = None, right: int | None = 0, sinks: int = 0,
                               key_mask: torch.Tensor | None = None, scale: float | None = None) -> tuple:
     """The gradients (dq, dk, dv) of `window_attention_forward` at dout like out."""
-    a, kept = _attn_args(q, k, v, left, right, sinks, key_mask, scale)
+    a, _kept = _attn_args(q, k, v, left, right, sinks, key_mask, scale)
     if dout.shape != q.shape or dout.dtype != q.dtype or out.shape != q.shape or out.dtype != q.dtype:
         _fail("dout and out must be like q")
     if lse.shape != (a.B, a.H, a.S) or lse.dtype != torch.float32:
@@ -312,10 +289,9 @@ def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
     a.dout, a.out, a.lse = dout.data_ptr(), out.data_ptr(), lse.data_ptr()
     a.do_sb, a.do_ss, a.do_sh = dout.stride()[:3]
     a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-    work = _bytes("d8s_attention_workspace", a, q.device)
+    work = hip.work_buffer("d8s_attention_workspace", q.device, a)
     a.workspace, a.ws_bytes = work.data_ptr(), work.numel()
-    _launch("d8s_attention_backward", a, q.device)
-    del kept
+    hip.launch("d8s_attention_backward", q.device, a)
     return dq, dk, dv
 
 
@@ -372,14 +348,10 @@ def window_attention_token(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
         _fail("the caches' channels must be contiguous")
     q, lengths = _last(q), lengths.contiguous()
-    a = hip.TokenArgs()
-    a.q, a.k, a.v, a.lengths, a.out = (t.data_ptr() for t in (q, k_cache, v_cache, lengths, out))
-    a.q_sb, a.q_sh = q.stride()[:2]
-    a.k_sb, a.k_ss, a.k_sh = k_cache.stride()[:3]
-    a.v_sb, a.v_ss, a.v_sh = v_cache.stride()[:3]
-    a.B, a.S, a.H, a.HK, a.D, a.dtype, a.scale = B, k_cache.shape[1], H, HK, D, hip.ELEMENTS[q.dtype], scale
-    a.left, a.sinks = _extent(left, "left"), _extent(sinks, "sinks")
-    work = _bytes("d8s_attention_token_workspace", a, q.device)
+    a = hip.TokenArgs(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lengths.data_ptr(), out.data_ptr(), 0, 0,
+                      *q.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3], B, k_cache.shape[1], H, HK, D,
+                      hip.ELEMENTS[q.dtype], _extent(left, "left"), _extent(sinks, "sinks"), scale, 0)
+    work = hip.work_buffer("d8s_attention_token_workspace", q.device, a)
     a.workspace, a.ws_bytes = work.data_ptr(), work.numel()
-    _launch("d8s_attention_token", a, q.device)
+    hip.launch("d8s_attention_token", q.device, a)
     return out

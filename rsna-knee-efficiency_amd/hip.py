@@ -340,6 +340,49 @@ def call(name: str, *args) -> None:
     check(getattr(library(), name)(*args), name)
 
 
+_ENTRIES: dict = {}
+# the current stream's handle without a Stream object around it, where this torch has the call
+_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def entry(name: str):
+    """Entry point `name`, looked up once per process (after the library's checks)."""
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        fn = _ENTRIES[name] = getattr(library(), name)
+    return fn
+
+
+def raw_stream(index: int) -> int:
+    """The hipStream_t of device `index`'s current stream."""
+    return _RAW_STREAM(index) if _RAW_STREAM is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def launch(name: str, device: torch.device, *args) -> None:
+    """Calls entry point `name` with `args` and then the current stream of `device`, which is made current for it."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = entry(name)(*args, raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = entry(name)(*args, raw_stream(index))
+    if rc:
+        check(rc, name)
+
+
+def work_buffer(name: str, device: torch.device, args) -> torch.Tensor:
+    """Device memory of as many bytes as entry point `name` says a call with `args` needs (at least one)."""
+    need = u64()
+    if torch.cuda.current_device() == device.index:
+        rc = entry(name)(args, need)
+    else:
+        with torch.cuda.device(device.index):
+            rc = entry(name)(args, need)
+    if rc:
+        check(rc, name)
+    return torch.empty(max(1, need.value), dtype=torch.uint8, device=device)
+
+
 def written(*tensors) -> None:
     """Marks tensors a kernel wrote through a raw pointer as modified: bumps their version counter
     (shared with their base and views), as an in-place torch op would, so a later consumer that

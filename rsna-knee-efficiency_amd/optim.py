@@ -10,8 +10,6 @@ the library the calls raise.
 """
 from __future__ import annotations
 
-import ctypes
-
 import numpy as np
 import torch
 
@@ -62,7 +60,8 @@ class AdamW:
                            "m_scale": zeros(total // block, torch.float32), "v_scale": zeros(total // block, torch.float32)}
         else:
             self._state = {"m": zeros(total, torch.float32), "v": zeros(total, torch.float32)}
-        self._dtypes = [p.dtype for p in self.params]
+        # what a step checks its tensors against
+        self._shapes, self._dtypes = [p.shape for p in self.params], [p.dtype for p in self.params]
 
     def _check(self, p: torch.Tensor) -> None:
         if p.dtype not in hip.ELEMENTS or not p.is_contiguous() or p.device != self.device or p.device.type != "cuda":
@@ -76,45 +75,42 @@ class AdamW:
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
             raise ValueError("a gradient (or None) for every parameter is required")
-        stream = torch.cuda.current_stream(self.device)
-        if hip.capturing(stream):
+        if torch.cuda.current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self._step(grads, grad_scale)
+        return self._step(grads, grad_scale)
+
+    def _step(self, grads: list, grad_scale: torch.Tensor | None) -> None:
+        if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("an optimizer step cannot be recorded into a graph")
         if grad_scale is not None and (grad_scale.numel() != 1 or grad_scale.dtype != torch.float32
                                        or grad_scale.device != self.device):
             raise ValueError("grad_scale must be one float32 on the parameters' GPU")
-        kinds: dict[tuple, list[int]] = {}
-        kept = []                              # (copies live until the launches are enqueued)
-        for i, (p, g) in enumerate(zip(self.params, grads)):
-            if g is None:
-                continue
-            if g.shape != p.shape or g.device != self.device:
-                raise ValueError(f"gradient {i} must have its parameter's shape and device")
-            if p.dtype != self._dtypes[i] or p.numel() != self._table["n"][i] or not p.is_contiguous():
-                raise ValueError(f"parameter {i} has changed")
-            if g.dtype not in hip.ELEMENTS or not (g.dtype == p.dtype or torch.float32 in (g.dtype, p.dtype)):
-                raise ValueError(f"gradient {i}: {g.dtype} beside {p.dtype}")
-            if not g.is_contiguous():
-                g = g.contiguous()
-                kept.append(g)
-            kinds.setdefault((p.dtype, g.dtype), []).append(i)
-            self._table["p"][i], self._table["g"][i] = p.data_ptr(), g.data_ptr()
+        params, shapes, dtypes, table, which = self.params, self._shapes, self._dtypes, self._table, None
+        if any(g is None for g in grads):
+            which = [i for i, g in enumerate(grads) if g is not None]
+            params, grads, shapes, dtypes = ([x[i] for i in which] for x in (params, grads, shapes, dtypes))
+            table = table[which]
+        if [p.shape for p in params] != shapes or [p.dtype for p in params] != dtypes or not all(p.is_contiguous() for p in params):
+            raise ValueError("a parameter has changed")
+        if [g.shape for g in grads] != shapes or any(g.device != self.device for g in grads):
+            raise ValueError("a gradient must have its parameter's shape and device")
+        kinds = list(zip(dtypes, [g.dtype for g in grads]))
+        for pt, gt in set(kinds):
+            if gt not in hip.ELEMENTS or not (gt == pt or torch.float32 in (gt, pt)):
+                raise ValueError(f"a gradient of {gt} beside a parameter of {pt}")
+        grads = [g if g.is_contiguous() else g.contiguous() for g in grads]     # (held until the launches are made)
+        table["p"], table["g"] = [p.data_ptr() for p in params], [g.data_ptr() for g in grads]
         s = self._state
-        a = hip.AdamwArgs()
-        if self.state_bits == 8:
-            a.m, a.v, a.m_scale, a.v_scale = (s[n].data_ptr() for n in ("m_code", "v_code", "m_scale", "v_scale"))
-        else:
-            a.m, a.v = s["m"].data_ptr(), s["v"].data_ptr()
-        a.grad_scale = 0 if grad_scale is None else grad_scale.data_ptr()
-        a.step, a.bits = self.step_count + 1, self.state_bits
-        a.lr, a.beta1, a.beta2, a.eps, a.weight_decay = self.lr, *self.betas, self.eps, self.weight_decay
-        with torch.cuda.device(self.device):
-            for (pt, gt), which in kinds.items():
-                rows = self._table if len(which) == len(self.params) else self._table[which]
-                a.tensors, a.count = rows.ctypes.data, len(rows)
-                a.dtype, a.grad_dtype = hip.ELEMENTS[pt], hip.ELEMENTS[gt]
-                hip.call("d8s_adamw", ctypes.byref(a), ctypes.c_void_p(stream.cuda_stream))
+        at = [t.data_ptr() for t in s.values()] + [0] * (4 - len(s))
+        for kind in dict.fromkeys(kinds):
+            rows = table if kinds.count(kind) == len(kinds) else table[[i for i, x in enumerate(kinds) if x == kind]]
+            hip.launch("d8s_adamw", self.device, hip.AdamwArgs(
+                rows.ctypes.data, *at, 0 if grad_scale is None else grad_scale.data_ptr(), self.step_count + 1, self.lr,
+                *self.betas, self.eps, self.weight_decay, len(rows), hip.ELEMENTS[kind[0]], hip.ELEMENTS[kind[1]],
+                self.state_bits))
         self.step_count += 1
-        hip.written(*(self.params[i] for which in kinds.values() for i in which), *s.values())
+        torch.autograd.graph.increment_version([*params, *s.values()])
 
     def moments(self) -> tuple[torch.Tensor, torch.Tensor]:
         """Both moments of all tensors, (elements,) float32, laid out as the state is: the state's own arrays, or
@@ -123,9 +119,8 @@ class AdamW:
         if self.state_bits == 32:
             return s["m"], s["v"]
         m, v = (torch.empty(s["m_code"].numel(), dtype=torch.float32, device=self.device) for _ in range(2))
-        with torch.cuda.device(self.device):
-            hip.call("d8s_adamw_moments", *(s[n].data_ptr() for n in ("m_code", "v_code", "m_scale", "v_scale")),
-                     m.numel(), m.data_ptr(), v.data_ptr(), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        hip.launch("d8s_adamw_moments", self.device, *(t.data_ptr() for t in s.values()), m.numel(), m.data_ptr(),
+                   v.data_ptr())
         return m, v
 
     def zero_grad(self) -> None:
