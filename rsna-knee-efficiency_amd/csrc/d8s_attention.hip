@@ -780,26 +780,46 @@ __global__ __launch_bounds__(NT) void k_token(D8sTokenArgs p, int split, float* 
     }
 }
 
+// A head's shares joined: their statistics by every wave, their sums by 256 / D groups of threads
 template <class T, int D>
-__global__ __launch_bounds__(D) void k_join(const float* part, T* out, int split, int heads) {
-    const int head = blockIdx.x, d = threadIdx.x;
-    float top = -INFINITY, o = 0.0f, sum = 0.0f;
-    for (int s = 0; s < split; ++s) top = fmaxf(top, part[((int64_t)s * heads + head) * (D + 2)]);
-    for (int s = 0; s < split; ++s) {
-        const float* t = part + ((int64_t)s * heads + head) * (D + 2);
-        const float a = t[0] == -INFINITY ? 0.0f : exp2_(t[0] - top);
-        sum = __builtin_fmaf(t[1], a, sum);
-        o = __builtin_fmaf(t[2 + d], a, o);
+__global__ __launch_bounds__(NT) void k_join(const float* part, T* out, int split, int heads) {
+    constexpr int GROUPS = NT / D;
+    __shared__ float so[GROUPS][D], ss[GROUPS];
+    const int head = blockIdx.x, d = threadIdx.x % D, g = threadIdx.x / D, lane = threadIdx.x % 64;
+    const float* p = part + (int64_t)head * (D + 2);
+    const int64_t step = (int64_t)heads * (D + 2);
+    float top = -INFINITY;
+    for (int s = lane; s < split; s += 64) top = fmaxf(top, p[s * step]);
+#pragma unroll
+    for (int x = 32; x >= 1; x /= 2) top = fmaxf(top, __shfl_xor(top, x));
+    float o = 0.0f, sum = 0.0f;
+#pragma unroll 8
+    for (int s = g; s < split; s += GROUPS) {
+        const float m = p[s * step], a = m == -INFINITY ? 0.0f : exp2_(m - top);
+        sum = __builtin_fmaf(p[s * step + 1], a, sum);
+        o = __builtin_fmaf(p[s * step + 2 + d], a, o);
+    }
+    so[g][d] = o;
+    if (d == 0) ss[g] = sum;
+    __syncthreads();
+    if (g != 0) return;
+    sum = ss[0];
+#pragma unroll
+    for (int x = 1; x < GROUPS; ++x) {
+        o += so[x][d];
+        sum += ss[x];
     }
     out[(int64_t)head * D + d] = (T)(sum > 0.0f || sum != sum ? o / sum : 0.0f);
 }
 
-// Shares of a token's keys: enough workgroups for two a compute unit, at least 64 keys each
+// Shares of a token's keys: enough workgroups for `TOKEN_WGS` a compute unit, at least the keys of one turn of a
+// workgroup's waves each
+constexpr int TOKEN_WGS = 4;
 int token_split(const D8sTokenArgs* a) {
-    const int G = a->H / a->HK, gm = G >= 8 ? 8 : G > 4 ? 8 : G > 2 ? 4 : G;
+    const int G = a->H / a->HK, gm = G > 4 ? 8 : G > 2 ? 4 : G;
     const int64_t problems = (int64_t)a->B * a->HK * ((G + gm - 1) / gm);
     const int64_t seen = std::min<int64_t>(a->S, (int64_t)a->left + 1 + a->sinks);
-    return (int)std::max<int64_t>(1, std::min((2 * d8s_host_cu_count() + problems - 1) / problems, seen / 64));
+    return (int)std::max<int64_t>(1, std::min((TOKEN_WGS * d8s_host_cu_count() + problems - 1) / problems, seen / (a->D == 64 ? 128 : 64)));
 }
 
 template <class T, int D>
@@ -815,7 +835,7 @@ void token_run(const D8sTokenArgs& a, hipStream_t st) {
     else if (G <= 4) go(k_token<T, D, 4>, 4);
     else go(k_token<T, D, 8>, 8);
     if (split > 1)
-        hipLaunchKernelGGL((k_join<T, D>), dim3((unsigned)(a.B * a.H)), dim3(D), 0, st, part, (T*)a.out, split, a.B * a.H);
+        hipLaunchKernelGGL((k_join<T, D>), dim3((unsigned)(a.B * a.H)), dim3(NT), 0, st, part, (T*)a.out, split, a.B * a.H);
 }
 
 // The arguments with a window no wider than the tokens (the kernels add its sides to positions)
