@@ -338,17 +338,43 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
     store_rows<T, ND>((T*)p.out + (((int64_t)b * p.S + i) * p.H + h) * D, acc, any ? 1.0f / l : 0.0f, i < p.S, lane);
 }
 
-// ---- backward: queries ------------------------------------------------------------------------------
-// As the forward pass, with do beside q: P from lse, dP = do v^T transposed, dS, dq += dS k.  It also leaves
-// rowsum(do o) for the keys' kernel.
+// ---- backward ----------------------------------------------------------------------------------------
+// k_attn_delta leaves rowsum(do o) of every query.  One launch then runs both kinds of workgroups beside each other:
+// first those of the keys (dk and dv, the longer ones), then those of the queries (dq), which fill the compute units
+// that the keys leave; what either writes the other does not read.  Both form s and dP again: a third product more
+// than sums shared through atomics would take, for results that do not depend on an order.
+template <class T, int D>
+__global__ __launch_bounds__(NT) void k_attn_delta(D8sAttnArgs p, float* delta) {
+    constexpr int L = D / 8, ROWS = NT / L;    // lanes a row, rows a workgroup
+    const int runs = (p.S + ROWS - 1) / ROWS;
+    const int run = blockIdx.x % runs, h = blockIdx.x / runs % p.H, b = blockIdx.x / runs / p.H;
+    const int i = run * ROWS + threadIdx.x / L, d = threadIdx.x % L * 8;
+    const int64_t ic = min(i, p.S - 1);
+    float g[8], o[8], x = 0.0f;
+    load_n<T, 8>((const T*)p.dout + b * p.do_sb + h * p.do_sh + ic * p.do_ss + d, 8, g);
+    load_n<T, 8>((const T*)p.out + (((int64_t)b * p.S + ic) * p.H + h) * D + d, 8, o);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x = __builtin_fmaf(g[k], o[k], x);
+    x = lanes_sum<L>(x);
+    if (d == 0 && i < p.S) delta[((int64_t)b * p.H + h) * p.S + i] = x;
+}
+
+// A tile's LDS: two buffers of two tiles of 64 rows, and of a float and another for each row
+template <int D>
+struct Shared {
+    u32x4 a[2][TILE * D / 8], b[2][TILE * D / 8];
+    float e[2][TILE], d[2][TILE];
+};
+
+// Queries: as the forward pass, with do beside q: P from lse, dP = do v^T transposed, dS, dq += dS k.
 DEV float lse2_of(float lse) { return lse == -INFINITY ? INFINITY : lse * LOG2E; }   // (empty row: every P is 0)
 
 template <class T, int D>
-__global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn_dq(D8sAttnArgs p, float* delta) {
+DEV void dq_body(const D8sAttnArgs& p, const float* delta, int id, Shared<D>& lds) {
     constexpr int ND = D / 32;
-    __shared__ u32x4 lk[2][TILE * D / 8], lv[2][TILE * D / 8];
+    auto &lk = lds.a, &lv = lds.b;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int nq = (p.S + 127) / 128, id = xcd_order(blockIdx.x, gridDim.x);
+    const int nq = (p.S + 127) / 128;
     const int b = id / (nq * p.H), h = id / nq % p.H, i00 = id % nq * 128, i0 = i00 + 32 * wave;
     const int hk = h / (p.H / p.HK);
     const uint16_t* kp = (const uint16_t*)p.k + b * p.k_sb + hk * p.k_sh;
@@ -356,27 +382,18 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn_dq(D8sAttnArgs p
     const int i = i0 + lane % 32;
     const int64_t ic = min(i, p.S - 1);
     Frag<T> q[D / 16], g[D / 16];
-    float dl = 0.0f;
     {
         const int64_t at = 8 * (lane / 32);
         const uint16_t* qp = (const uint16_t*)p.q + b * p.q_sb + h * p.q_sh + ic * p.q_ss + at;
         const uint16_t* gp = (const uint16_t*)p.dout + b * p.do_sb + h * p.do_sh + ic * p.do_ss + at;
-        const uint16_t* op = (const uint16_t*)p.out + (((int64_t)b * p.S + ic) * p.H + h) * D + at;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
             q[k] = __builtin_bit_cast(Frag<T>, *(const Raw*)(qp + 16 * k));
             g[k] = __builtin_bit_cast(Frag<T>, *(const Raw*)(gp + 16 * k));
-            const Frag<T> o = __builtin_bit_cast(Frag<T>, *(const Raw*)(op + 16 * k));
-#pragma unroll
-            for (int j = 0; j < 8; ++j) dl = __builtin_fmaf((float)g[k][j], (float)o[j], dl);
         }
-        float a, c;
-        swap32(dl, a, c);
-        dl = a + c;
     }
     const int64_t stat = ((int64_t)b * p.H + h) * p.S + ic;
-    if (lane < 32 && i < p.S) delta[stat] = dl;
-    const float c = p.scale * LOG2E, lse2 = lse2_of(p.lse[stat]);
+    const float c = p.scale * LOG2E, lse2 = lse2_of(p.lse[stat]), dl = delta[stat];
     f32x16 acc[ND] = {};
     const Tiles tiles = tiles_of(p, i00, min(i00 + 127, p.S - 1));
     const Copy<D, TILE> copy;
@@ -434,57 +451,49 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn_dq(D8sAttnArgs p
     store_rows<T, ND>((T*)p.dq + (((int64_t)b * p.S + i) * p.H + h) * D, acc, p.scale, i < p.S, lane);
 }
 
-// ---- backward: keys and values ----------------------------------------------------------------------
-// A workgroup runs 128 KB keys of a key head, 32 KB a wave, over the tiles of 64 queries that see them, one query head
-// of the group after the other, so that dk and dv of shared heads are sums within one workgroup, in a fixed order.  The
+// Keys: a workgroup runs 128 keys of a key head, 32 a wave, over the tiles of 64 queries that see them, one query head of
+// the group after the other, so that dk and dv of shared heads are sums within one workgroup, in a fixed order.  The
 // tiles of the first tokens are seen by every query: their queries are split over `sink_split` workgroups (and all
 // tiles' over `split` where there are fewer tiles than compute units), whose float32 sums k_attn_join adds.
 // The products start from -lse / scale and -rowsum(do o) in place of zero, so P and dS are an exponential and a product.
 struct KeySplit {
     int sink_tiles, sink_split, split;
 };
-template <int D>
-constexpr int KB = 1;                          // blocks of 32 keys a wave
-template <int D>
-constexpr int KEYS = 128 * KB<D>;
+constexpr int KEYS = 128;
 
 template <class T, int D>
-__global__ __launch_bounds__(NT, 2) void k_attn_dkv(D8sAttnArgs p, const float* delta, float* part, KeySplit ks) {
-    constexpr int ND = D / 32, NB = KB<D>;
-    __shared__ u32x4 lq[2][TILE * D / 8], lg[2][TILE * D / 8];
-    __shared__ float ls[2][TILE], ld[2][TILE];
+DEV void dkv_body(const D8sAttnArgs& p, const float* delta, float* part, KeySplit ks, int id, Shared<D>& lds) {
+    constexpr int ND = D / 32;
+    auto &lq = lds.a, &lg = lds.b;
+    auto &ls = lds.e, &ld = lds.d;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int nk = (p.S + KEYS<D> - 1) / KEYS<D>, G = p.H / p.HK;
+    const int nk = (p.S + KEYS - 1) / KEYS, G = p.H / p.HK;
     const int items = ks.sink_tiles * ks.sink_split + (nk - ks.sink_tiles) * ks.split;
-    const int id = xcd_order(blockIdx.x, gridDim.x), item = id % items, bh = id / items, b = bh / p.HK, hk = bh % p.HK;
+    const int item = id % items, bh = id / items, b = bh / p.HK, hk = bh % p.HK;
     const bool sink = item < ks.sink_tiles * ks.sink_split;
     const int rest = sink ? item : item - ks.sink_tiles * ks.sink_split, n = sink ? ks.sink_split : ks.split;
     const int kt = (sink ? 0 : ks.sink_tiles) + rest / n, cut = rest % n;
-    const int j0 = kt * KEYS<D>, jw = j0 + 32 * NB * wave, jl = jw + lane % 32;
+    const int j0 = kt * KEYS, jw = j0 + 32 * wave, j = jw + lane % 32;
     const uint8_t* mask = p.mask ? p.mask + b * p.mask_sb : nullptr;
-    bool on[NB], any = false;
-    Frag<T> k[NB][D / 16], v[NB][D / 16];
-#pragma unroll
-    for (int y = 0; y < NB; ++y) {
-        const int64_t jc = min(jl + 32 * y, p.S - 1);
-        on[y] = jl + 32 * y < p.S && (mask == nullptr || mask[jc] != 0);
-        any |= on[y];
+    const int64_t jc = min(j, p.S - 1);
+    const bool on = j < p.S && (mask == nullptr || mask[jc] != 0), any = __any(on);
+    Frag<T> k[D / 16], v[D / 16];
+    {
         const uint16_t* kp = (const uint16_t*)p.k + b * p.k_sb + hk * p.k_sh + jc * p.k_ss + 8 * (lane / 32);
         const uint16_t* vp = (const uint16_t*)p.v + b * p.v_sb + hk * p.v_sh + jc * p.v_ss + 8 * (lane / 32);
 #pragma unroll
         for (int u = 0; u < D / 16; ++u) {
-            k[y][u] = __builtin_bit_cast(Frag<T>, *(const Raw*)(kp + 16 * u));
-            v[y][u] = __builtin_bit_cast(Frag<T>, *(const Raw*)(vp + 16 * u));
+            k[u] = __builtin_bit_cast(Frag<T>, *(const Raw*)(kp + 16 * u));
+            v[u] = __builtin_bit_cast(Frag<T>, *(const Raw*)(vp + 16 * u));
         }
     }
-    any = __any(any);
     // queries that see any of the keys: from j0 - right, to left past the last key or the end for a first token
     const int lo = max(0, j0 - p.right) / TILE;
-    const int hi = (j0 < p.sinks ? p.S - 1 : min(p.S - 1, j0 + KEYS<D> - 1 + p.left)) / TILE;
+    const int hi = (j0 < p.sinks ? p.S - 1 : min(p.S - 1, j0 + KEYS - 1 + p.left)) / TILE;
     const int per = hi - lo + 1;
     const int t0 = (int)((int64_t)G * per * cut / n), t1 = (int)((int64_t)G * per * (cut + 1) / n);
     const float c = p.scale * LOG2E, c1 = 1.0f / p.scale;
-    f32x16 dk[NB][ND] = {}, dv[NB][ND] = {};
+    f32x16 dk[ND] = {}, dv[ND] = {};
     const Copy<D, TILE> copy;
     float se = 0.0f, sd = 0.0f;
     int h = hk * G + t0 / per, qt = lo + t0 % per;         // of the tile whose copies are on their way
@@ -521,107 +530,90 @@ __global__ __launch_bounds__(NT, 2) void k_attn_dkv(D8sAttnArgs p, const float* 
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int q0 = qn + 32 * u;
-            if (q0 >= p.S || none_seen(p, q0, jw, jw + 32 * NB - 1)) continue;
-            f32x16 s[NB], dp[NB];
+            if (q0 >= p.S || none_seen(p, q0, jw, jw + 31)) continue;
+            f32x16 s, dp;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const f32x4 e = *(const f32x4*)&ls[buf][32 * u + 8 * g + 4 * (lane / 32)];
                 const f32x4 d = *(const f32x4*)&ld[buf][32 * u + 8 * g + 4 * (lane / 32)];
 #pragma unroll
-                for (int y = 0; y < NB; ++y)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        s[y][4 * g + r] = e[r];
-                        dp[y][4 * g + r] = d[r];
-                    }
+                for (int r = 0; r < 4; ++r) {
+                    s[4 * g + r] = e[r];
+                    dp[4 * g + r] = d[r];
+                }
             }
 #pragma unroll
             for (int x = 0; x < D / 16; ++x) {
-                const Frag<T> fq = rows_frag<T, D>(rq, 32 * u, x), fg = rows_frag<T, D>(rg, 32 * u, x);
-#pragma unroll
-                for (int y = 0; y < NB; ++y) {
-                    s[y] = mfma(fq, k[y][x], s[y]);
-                    dp[y] = mfma(fg, v[y][x], dp[y]);
-                }
+                s = mfma(rows_frag<T, D>(rq, 32 * u, x), k[x], s);
+                dp = mfma(rows_frag<T, D>(rg, 32 * u, x), v[x], dp);
             }
 #pragma unroll
-            for (int y = 0; y < NB; ++y)
+            for (int r = 0; r < 16; ++r) {
+                s[r] = exp2_(s[r] * c);
+                dp[r] *= s[r];
+            }
+            if (!all_seen(p, q0, jw, jw + 31)) {
+                // query q0 + r sees key j: r >= j - right - q0, and r <= j + left - q0 or j is a first token
+                const uint64_t vis = bits_from(j - p.right - q0) & (j < p.sinks ? ~0ull : bits_below(j + p.left + 1 - q0));
+                const uint32_t mine = lane_rows((uint32_t)vis, lane);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    s[y][r] = exp2_(s[y][r] * c);
-                    dp[y][r] *= s[y][r];
-                }
-            if (!all_seen(p, q0, jw, jw + 32 * NB - 1)) {
-#pragma unroll
-                for (int y = 0; y < NB; ++y) {
-                    // query q0 + r sees key j: r >= j - right - q0, and r <= j + left - q0 or j is a first token
-                    const int j = jl + 32 * y;
-                    const uint64_t vis = bits_from(j - p.right - q0) & (j < p.sinks ? ~0ull : bits_below(j + p.left + 1 - q0));
-                    const uint32_t mine = lane_rows((uint32_t)vis, lane);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const uint32_t keep = keep_mask(mine, r);
-                        s[y][r] = __uint_as_float(__float_as_uint(s[y][r]) & keep);
-                        dp[y][r] = __uint_as_float(__float_as_uint(dp[y][r]) & keep);
-                    }
+                    const uint32_t keep = keep_mask(mine, r);
+                    s[r] = __uint_as_float(__float_as_uint(s[r]) & keep);
+                    dp[r] = __uint_as_float(__float_as_uint(dp[r]) & keep);
                 }
             }
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-                Frag<T> pf[NB], df[NB];
-#pragma unroll
-                for (int y = 0; y < NB; ++y) {
-                    pf[y] = round_frag<T>(s[y], w);
-                    df[y] = round_frag<T>(dp[y], w);
-                }
+                const Frag<T> pf = round_frag<T>(s, w), df = round_frag<T>(dp, w);
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    const Frag<T> fg = cols_frag<T, D>(cg, 32 * u + 16 * w, d), fq = cols_frag<T, D>(cq, 32 * u + 16 * w, d);
-#pragma unroll
-                    for (int y = 0; y < NB; ++y) {
-                        dv[y][d] = mfma(fg, pf[y], dv[y][d]);
-                        dk[y][d] = mfma(fq, df[y], dk[y][d]);
-                    }
+                    dv[d] = mfma(cols_frag<T, D>(cg, 32 * u + 16 * w, d), pf, dv[d]);
+                    dk[d] = mfma(cols_frag<T, D>(cq, 32 * u + 16 * w, d), df, dk[d]);
                 }
             }
         }
     }
+    if (!on) {                                 // a masked key's column may hold anything: it has no gradient
 #pragma unroll
-    for (int y = 0; y < NB; ++y) {
-        const int j = jl + 32 * y;
-        if (!on[y]) {                          // a masked key's column may hold anything: it has no gradient
-#pragma unroll
-            for (int d = 0; d < ND; ++d) dk[y][d] = dv[y][d] = f32x16{};
-        }
-        if (n > 1) {                           // part[problem and item][dk, dv][key][D]
-            float* o = part + (int64_t)id * 2 * KEYS<D> * D + (int64_t)(j - j0) * D + 4 * (lane / 32);
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    f32x4 x, z;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        x[r] = dk[y][d][4 * g + r] * p.scale;
-                        z[r] = dv[y][d][4 * g + r];
-                    }
-                    if (j < p.S) {
-                        *(f32x4*)(o + 32 * d + 8 * g) = x;
-                        *(f32x4*)(o + KEYS<D> * D + 32 * d + 8 * g) = z;
-                    }
-                }
-        } else {
-            const int64_t at = (((int64_t)b * p.S + j) * p.HK + hk) * D;
-            store_rows<T, ND>((T*)p.dk + at, dk[y], p.scale, j < p.S, lane);
-            store_rows<T, ND>((T*)p.dv + at, dv[y], 1.0f, j < p.S, lane);
-        }
+        for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
     }
+    if (n > 1) {                               // part[problem and item][dk, dv][key][D]
+        if (j >= p.S) return;
+        float* o = part + (int64_t)id * 2 * KEYS * D + (int64_t)(j - j0) * D + 4 * (lane / 32);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                f32x4 x, z;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = dk[d][4 * g + r] * p.scale;
+                    z[r] = dv[d][4 * g + r];
+                }
+                *(f32x4*)(o + 32 * d + 8 * g) = x;
+                *(f32x4*)(o + KEYS * D + 32 * d + 8 * g) = z;
+            }
+        return;
+    }
+    const int64_t at = (((int64_t)b * p.S + j) * p.HK + hk) * D;
+    store_rows<T, ND>((T*)p.dk + at, dk, p.scale, j < p.S, lane);
+    store_rows<T, ND>((T*)p.dv + at, dv, 1.0f, j < p.S, lane);
+}
+
+// The first `of_keys` workgroups run keys, the others queries
+template <class T, int D>
+__global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn_back(D8sAttnArgs p, const float* delta, float* part, KeySplit ks,
+                                                                     int of_keys) {
+    __shared__ Shared<D> lds;
+    const int w = blockIdx.x;
+    if (w < of_keys) dkv_body<T, D>(p, delta, part, ks, xcd_order(w, of_keys), lds);
+    else dq_body<T, D>(p, delta, xcd_order(w - of_keys, gridDim.x - of_keys), lds);
 }
 
 // dk and dv of the split tiles: the float32 parts summed in order, four values a thread
 template <class T, int D>
 __global__ __launch_bounds__(NT) void k_attn_join(D8sAttnArgs p, const float* part, KeySplit ks) {
-    constexpr int KEYS = 128 * KB<D>;
     const int nk = (p.S + KEYS - 1) / KEYS, items = ks.sink_tiles * ks.sink_split + (nk - ks.sink_tiles) * ks.split;
     const int joined = ks.split > 1 ? nk : ks.sink_tiles;          // tiles per problem, the first ones
     const int kt = blockIdx.x % joined, bh = blockIdx.x / joined, b = bh / p.HK, hk = bh % p.HK;
@@ -639,18 +631,25 @@ __global__ __launch_bounds__(NT) void k_attn_join(D8sAttnArgs p, const float* pa
     store_n<T, 4>(o, 4, f);
 }
 
+// Into how many workgroups a key tile's queries are split.  In units of one tile of 64 queries for one wave of keys (a
+// tile of queries for dq counts the same), a workgroup gets at most its share of all work on the slots of the GPU, at
+// least eight units (a shorter one is mostly beginning and end) and, unless its keys are first tokens, whole tiles
+// where there are enough of them.
 KeySplit key_split(const D8sAttnArgs* a) {
-    const int64_t S = a->S, keys = a->D == 64 ? KEYS<64> : KEYS<128>, nk = (S + keys - 1) / keys, nq = (S + 63) / 64, G = a->H / a->HK;
-    const int64_t seen = std::min(nq, (std::min<int64_t>(a->left, S) + std::min<int64_t>(a->right, S) + keys) / 64 + 1);
-    const int64_t cus = d8s_host_cu_count(), problems = (int64_t)a->B * a->HK;
+    const int64_t S = a->S, nk = (S + KEYS - 1) / KEYS, nq = (S + TILE - 1) / TILE, G = a->H / a->HK;
+    const int64_t wide = std::min<int64_t>(a->left, S) + std::min<int64_t>(a->right, S);
+    const int64_t seen = std::min(nq, (wide + KEYS) / TILE + 1), problems = (int64_t)a->B * a->HK;
+    const int64_t slots = (int64_t)d8s_host_cu_count() * (a->D == 64 ? 3 : 2);
+    const int64_t all = problems * nk * G * seen * 2;
+    const int64_t most = std::max<int64_t>(8, std::min(G * seen, all / slots));
     KeySplit k;
-    k.split = (int)std::max<int64_t>(1, std::min(cus / std::max<int64_t>(1, problems * nk), G * seen / 4));
-    k.sink_tiles = (int)std::min(nk, ((int64_t)a->sinks + keys - 1) / keys);
-    k.sink_split = (int)std::min<int64_t>(G * nq, (k.split * nq + seen - 1) / seen);
+    k.split = (int)((G * seen + most - 1) / most);
+    k.sink_tiles = (int)std::min(nk, ((int64_t)a->sinks + KEYS - 1) / KEYS);
+    k.sink_split = (int)((G * nq + most - 1) / most);
     return k;
 }
 int64_t key_items(const D8sAttnArgs* a, const KeySplit& k) {
-    const int keys = a->D == 64 ? KEYS<64> : KEYS<128>, nk = (a->S + keys - 1) / keys;
+    const int64_t nk = (a->S + KEYS - 1) / KEYS;
     return (int64_t)k.sink_tiles * k.sink_split + (nk - k.sink_tiles) * k.split;
 }
 uint64_t delta_bytes(const D8sAttnArgs* a) { return ((uint64_t)a->B * a->H * a->S * 4 + 255) / 256 * 256; }
@@ -858,12 +857,14 @@ void attn_back_run(const D8sAttnArgs& a, hipStream_t st) {
     float* delta = (float*)a.workspace;
     float* part = (float*)((char*)a.workspace + delta_bytes(&a));
     const KeySplit ks = key_split(&a);
-    const unsigned grid = (unsigned)((int64_t)a.B * a.H * ((a.S + 127) / 128));
-    const int problems = a.B * a.HK, nk = (a.S + KEYS<D> - 1) / KEYS<D>, joined = ks.split > 1 ? nk : ks.sink_split > 1 ? ks.sink_tiles : 0;
-    hipLaunchKernelGGL((k_attn_dq<T, D>), dim3(grid), dim3(NT), 0, st, a, delta);
-    hipLaunchKernelGGL((k_attn_dkv<T, D>), dim3((unsigned)(problems * key_items(&a, ks))), dim3(NT), 0, st, a, delta, part, ks);
+    const int problems = a.B * a.HK, nk = (a.S + KEYS - 1) / KEYS;
+    const int joined = ks.split > 1 ? nk : ks.sink_split > 1 ? ks.sink_tiles : 0;
+    const int of_keys = problems * (int)key_items(&a, ks), of_queries = a.B * a.H * ((a.S + 127) / 128);
+    constexpr int ROWS = NT / (D / 8);
+    hipLaunchKernelGGL((k_attn_delta<T, D>), dim3((unsigned)(a.B * a.H * ((a.S + ROWS - 1) / ROWS))), dim3(NT), 0, st, a, delta);
+    hipLaunchKernelGGL((k_attn_back<T, D>), dim3((unsigned)(of_keys + of_queries)), dim3(NT), 0, st, a, delta, part, ks, of_keys);
     if (joined)
-        hipLaunchKernelGGL((k_attn_join<T, D>), dim3((unsigned)(problems * joined), 2 * KEYS<D> * D / (4 * NT)), dim3(NT), 0, st,
+        hipLaunchKernelGGL((k_attn_join<T, D>), dim3((unsigned)(problems * joined), 2 * KEYS * D / (4 * NT)), dim3(NT), 0, st,
                            a, part, ks);
 }
 
@@ -881,7 +882,7 @@ int attn_check(const D8sAttnArgs* a, const char* what) {
     AREQ(a->S <= (1 << 29), "more than 2^29 tokens");
     AREQ((int64_t)a->B * a->H * ((a->S + 127) / 128) < (1 << 24), "too many heads and tokens");
     AREQ(a->left >= 0 && a->right >= 0 && a->sinks >= 0, "left, right and sinks must not be negative");
-    AREQ(a->scale > 0 && a->scale < INFINITY, "scale must be positive and finite");
+    AREQ(a->scale > 0 && a->scale < INFINITY && 1.0f / a->scale < INFINITY, "scale must be positive and finite, and 1 / scale too");
     AREQ(a->q && a->k && a->v && a->out, "null pointer");
     return 0;
 }
@@ -901,7 +902,7 @@ extern "C" int d8s_attention_workspace(const D8sAttnArgs* a, uint64_t* bytes) {
     AREQ(bytes != nullptr, "null arguments");
     const KeySplit k = key_split(a);
     const bool parts = k.split > 1 || (k.sink_tiles > 0 && k.sink_split > 1);
-    *bytes = delta_bytes(a) + (parts ? (uint64_t)a->B * a->HK * key_items(a, k) * 2 * (a->D == 64 ? KEYS<64> : KEYS<128>) * a->D * 4 : 0);
+    *bytes = delta_bytes(a) + (parts ? (uint64_t)a->B * a->HK * key_items(a, k) * 2 * KEYS * a->D * 4 : 0);
     return 0;
 }
 
@@ -913,7 +914,8 @@ extern "C" int d8s_attention_backward(const D8sAttnArgs* a, void* stream) {
     if (int rc = d8s_attention_workspace(a, &need)) return rc;
     AREQ(a->ws_bytes >= need && ((uintptr_t)a->workspace & 15) == 0,
          "workspace smaller than d8s_attention_workspace() or not 16-byte aligned");
-    AREQ((int64_t)a->B * a->HK * key_items(a, key_split(a)) < (1 << 24), "too many heads and tokens");
+    AREQ((int64_t)a->B * a->H * ((a->S + 15) / 16) + (int64_t)a->B * a->HK * key_items(a, key_split(a)) < (1 << 24),
+         "too many heads and tokens");
     BY_TYPE(attn_back_run, clipped(a), (hipStream_t)stream);
     return d8s_host_launched(what);
 }
@@ -925,7 +927,7 @@ static int token_check(const D8sTokenArgs* a, const char* what) {
     AREQ(a->B >= 1 && a->S >= 1 && a->H >= 1 && a->HK >= 1 && a->H % a->HK == 0, "bad sizes (H a multiple of HK)");
     AREQ((int64_t)a->B * a->H < (1 << 22), "too many heads");
     AREQ(a->left >= 0 && a->sinks >= 0, "left and sinks must not be negative");
-    AREQ(a->scale > 0 && a->scale < INFINITY, "scale must be positive and finite");
+    AREQ(a->scale > 0 && a->scale < INFINITY && 1.0f / a->scale < INFINITY, "scale must be positive and finite, and 1 / scale too");
     return 0;
 }
 
