@@ -633,7 +633,7 @@ __global__ __launch_bounds__(NT) void k_attn_join(D8sAttnArgs p, const float* pa
 
 // Into how many workgroups a key tile's queries are split.  In units of one tile of 64 queries for one wave of keys (a
 // tile of queries for dq counts the same), a workgroup gets at most its share of all work on the slots of the GPU, at
-// least eight units (a shorter one is mostly beginning and end) and, unless its keys are first tokens, whole tiles
+// least twelve units (a shorter one is mostly beginning and end) and, unless its keys are first tokens, whole tiles
 // where there are enough of them.
 KeySplit key_split(const D8sAttnArgs* a) {
     const int64_t S = a->S, nk = (S + KEYS - 1) / KEYS, nq = (S + TILE - 1) / TILE, G = a->H / a->HK;
@@ -641,7 +641,7 @@ KeySplit key_split(const D8sAttnArgs* a) {
     const int64_t seen = std::min(nq, (wide + KEYS) / TILE + 1), problems = (int64_t)a->B * a->HK;
     const int64_t slots = (int64_t)d8s_host_cu_count() * (a->D == 64 ? 3 : 2);
     const int64_t all = problems * nk * G * seen * 2;
-    const int64_t most = std::max<int64_t>(8, std::min(G * seen, all / slots));
+    const int64_t most = std::max<int64_t>(12, std::min(G * seen, all / slots));
     KeySplit k;
     k.split = (int)((G * seen + most - 1) / most);
     k.sink_tiles = (int)std::min(nk, ((int64_t)a->sinks + KEYS - 1) / KEYS);
