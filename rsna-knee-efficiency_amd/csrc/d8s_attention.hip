@@ -284,6 +284,9 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
 #pragma unroll
             for (int k = 1; k < D / 16; ++k) s[u] = mfma(rows_frag<T, D>(rk, 32 * u, k), q[k], s[u]);
         }
+        Frag<T> early[ND];                     // the first values, read while the exponentials are formed
+#pragma unroll
+        for (int d = 0; d < ND; ++d) early[d] = cols_frag<T, D>(cv, 0, d);
         if (bits != ~0ull || !all_seen(p, i0, now, now + TILE - 1)) {
             const uint64_t vis = bits & bits_below(i + p.right + 1 - now) & (bits_from(i - p.left - now) | bits_below(p.sinks - now));
 #pragma unroll
@@ -327,7 +330,7 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
         for (int u = 0; u < 4; ++u) {
             const Frag<T> w = round_frag<T>(s[u / 2], u % 2);
 #pragma unroll
-            for (int d = 0; d < ND; ++d) acc[d] = mfma(cols_frag<T, D>(cv, 16 * u, d), w, acc[d]);
+            for (int d = 0; d < ND; ++d) acc[d] = mfma(u == 0 ? early[d] : cols_frag<T, D>(cv, 16 * u, d), w, acc[d]);
         }
     }
     float l0, l1;

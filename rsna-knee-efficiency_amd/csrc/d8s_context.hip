@@ -226,7 +226,7 @@ int norm_rows(int width) { return width <= 128 ? 16 : width <= 2048 ? 4 : 1; }
 
 int norm_parts(const D8sNormArgs* a) {
     const int64_t per = norm_rows(a->width), all = (a->rows + per - 1) / per;
-    return (int)std::min<int64_t>(all, 2 * d8s_host_cu_count());
+    return (int)std::min<int64_t>(all, 4 * d8s_host_cu_count());
 }
 
 template <class T, class W, int TPR, int E>
