@@ -138,13 +138,30 @@ __global__ __launch_bounds__(256) void k_adamw(Table t, Step s) {
             float ms, mi, rs, ri;
             block_scale(mtop, ms, mi);
             block_scale(rtop, rs, ri);
+            // A code is a square root rounded to a whole number.  The hardware's root is within 2^-22 of the exactly
+            // rounded one, so the two give the same code unless the root lies within 2^-13 of a half, which is
+            // rare: then the wave rounds all of its block's codes from exact roots.  (The expansion of an exact root
+            // is a dozen operations, and the step was bound by its operations: 337 -> 299 us for 98 M elements.)
+            float mr[4], vr[4], worst = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float x = __builtin_amdgcn_sqrtf(fabsf(m[k]) * mi) * 127.0f, y = __builtin_amdgcn_sqrtf(r[k] * ri) * 255.0f;
+                mr[k] = rintf(x);
+                vr[k] = rintf(y);
+                worst = fmaxf(worst, fmaxf(fabsf(x - mr[k]), fabsf(y - vr[k])));
+            }
+            if (__any(!(worst < 0.5f - 0x1p-13f))) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    mr[k] = fminf(rintf(sqrtf(fabsf(m[k]) * mi) * 127.0f), 127.0f);
+                    vr[k] = fminf(rintf(sqrtf(r[k] * ri) * 255.0f), 255.0f);
+                }
+            }
             mc = vc = 0;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                int c = (int)fminf(rintf(sqrtf(fabsf(m[k]) * mi) * 127.0f), 127.0f);
-                c = m[k] < 0.0f ? -c : c;
-                int d = (int)fminf(rintf(sqrtf(r[k] * ri) * 255.0f), 255.0f);
-                d = d == 0 && r[k] > 0.0f && rs > 0.0f ? 1 : d;
+                const int c = (int)copysignf(mr[k], m[k]);
+                const int d = (int)(r[k] > 0.0f && rs > 0.0f ? fmaxf(vr[k], 1.0f) : vr[k]);
                 mc |= (uint32_t)(c & 255) << (8 * k);
                 vc |= (uint32_t)(d & 255) << (8 * k);
             }
