@@ -21,10 +21,18 @@ def _fail(message: str):
     raise ValueError(message)
 
 
-def _on_gpu(*tensors: torch.Tensor) -> None:
-    device = tensors[0].device
-    if device.type != "cuda" or any(t.device != device for t in tensors):
+def _on_gpu(first: torch.Tensor, *others: torch.Tensor) -> None:
+    index = first.get_device()                 # (an int, -1 on the CPU: a call has up to six tensors to look at)
+    if index < 0:
         _fail("the tensors must be on one GPU")
+    for t in others:
+        if t.get_device() != index:
+            _fail("the tensors must be on one GPU")
+
+
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """A new contiguous tensor of x's shape and type"""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
 
 
 # --- layer norm -----------------------------------------------------------------------------------
@@ -60,11 +68,12 @@ def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor
         _fail("bias must be like weight")
     device = x.device
     _on_gpu(x, weight, weight if bias is None else bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    y = _like(x)
     n = x.numel() // width
     mean = rstd = None
     if statistics:
-        mean, rstd = (torch.empty(n, dtype=torch.float32, device=device) for _ in range(2))
+        mean = x.new_empty(n, dtype=torch.float32)
+        rstd = torch.empty_like(mean)
     if n:
         rows, weight = _rows(x), weight.contiguous()
         bias = None if bias is None else bias.contiguous()
@@ -86,11 +95,11 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
         _fail("mean and rstd must be float32, one a row")
     device = x.device
     _on_gpu(x, dy, weight, mean, rstd)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=device)
+    dx = _like(x)
     if not n:
         return dx, torch.zeros_like(weight), torch.zeros_like(weight)
-    dw, db = (torch.empty(width, dtype=weight.dtype, device=device) for _ in range(2))
     rows, grad, weight, mean, rstd = _rows(x), _rows(dy), weight.contiguous(), mean.contiguous(), rstd.contiguous()
+    dw, db = torch.empty_like(weight), torch.empty_like(weight)
     a = hip.NormArgs(rows.data_ptr(), weight.data_ptr(), 0, 0, mean.data_ptr(), rstd.data_ptr(), grad.data_ptr(),
                      dx.data_ptr(), dw.data_ptr(), db.data_ptr(), 0, 0, n, rows.stride(0), grad.stride(0), width, dtype,
                      wdtype, 0.0)
@@ -155,7 +164,7 @@ def _rotate(x, positions, sections, base, adjacent, inverse, out):
     x = x if x.stride(3) == 1 else x.contiguous()
     positions = positions if positions.stride(-1) == 1 else positions.contiguous()
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _like(x)
     elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(3) != 1:
         _fail("out must be like x, its channels contiguous")
     if not x.numel():
@@ -264,8 +273,8 @@ def window_attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     -> (out like q, lse (batch, heads, tokens) float32: the logarithm of the sum of exponentials, -inf where nothing
     is seen; None without `statistics`)"""
     a, _kept = _attn_args(q, k, v, left, right, sinks, key_mask, scale)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((a.B, a.H, a.S), dtype=torch.float32, device=q.device) if statistics else None
+    out = _like(q)
+    lse = q.new_empty((a.B, a.H, a.S), dtype=torch.float32) if statistics else None
     if q.numel():
         a.out, a.lse = out.data_ptr(), lse.data_ptr() if statistics else 0
         hip.launch("d8s_attention", q.device, a)
@@ -282,7 +291,7 @@ def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
     if lse.shape != (a.B, a.H, a.S) or lse.dtype != torch.float32:
         _fail("lse must be (batch, heads, tokens) float32")
     _on_gpu(q, dout, out, lse)
-    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
+    dq, dk, dv = _like(q), _like(k), _like(v)
     if not q.numel():
         return dq, dk.zero_(), dv.zero_()
     dout, out, lse = _last(dout), out.contiguous(), lse.contiguous()
@@ -342,7 +351,7 @@ def window_attention_token(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 0 < scale < math.inf:
         _fail("scale must be positive and finite")
-    out = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
+    out = _like(q)
     if not out.numel() or not k_cache.shape[1]:
         return out.zero_()
     if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
