@@ -63,11 +63,11 @@ DEV int swizzle(int r) {
     }
 }
 
-// LDS by byte address: every address of a tile's operands is the lane's first one with some bits flipped (the piece)
-// and a constant added (the rows), so two registers serve all of them.
-typedef __attribute__((address_space(3))) char* lds_bytes;
-DEV uint32_t lds_at(const void* p) { return (uint32_t)(uintptr_t)(lds_bytes)p; }
-
+// Every address of a tile's operands is the lane's first one with some bits flipped (the piece) and a constant added
+// (the rows), so two registers serve all of them.
+// A tile's two buffers are shared arrays of their own, and a loop's turn names them: so the compiler sees that reads of
+// one do not wait for the copies into the other (through one array, or addresses as numbers, it waits for every copy
+// in flight before the first read: the copies of the next tile would be waited for at once).
 // The lane's first address for rows_frag, and for cols_frag, relative to a tile
 template <int D>
 DEV uint32_t rows_at(int lane) {
@@ -87,18 +87,17 @@ DEV uint32_t fresh(uint32_t at) {
 
 // Operand of rows r0 .. r0 + 31 (r0 a multiple of 16), values 16 k .. 16 k + 15 of each
 template <class T, int D>
-DEV Frag<T> rows_frag(uint32_t at, int r0, int k) {
-    typedef const __attribute__((address_space(3))) u32x4* lds;
-    return __builtin_bit_cast(Frag<T>, *(lds)(uintptr_t)((at ^ (uint32_t)(k << 5)) + r0 * 2 * D));
+DEV Frag<T> rows_frag(const u32x4* tile, uint32_t at, int r0, int k) {
+    return __builtin_bit_cast(Frag<T>, *(const u32x4*)((const char*)tile + ((at ^ (uint32_t)(k << 5)) + r0 * 2 * D)));
 }
 
 // Operand of columns 32 d .. 32 d + 31, summed over the tile's rows r0 .. r0 + 15 in the order of a result's registers
 template <class T, int D>
-DEV Frag<T> cols_frag(uint32_t at, int r0, int d) {
+DEV Frag<T> cols_frag(const u32x4* tile, uint32_t at, int r0, int d) {
     typedef __attribute__((address_space(3))) s16x4* lds;
     const uint32_t lo = at ^ (uint32_t)(d << 6), hi = lo ^ (D == 64 ? 16u : 32u);    // (8 rows on, the swizzle differs in one bit)
-    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(uintptr_t)(lo + r0 * 2 * D));
-    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(uintptr_t)(hi + (r0 + 8) * 2 * D));
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)((const char*)tile + (lo + r0 * 2 * D)));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)((const char*)tile + (hi + (r0 + 8) * 2 * D)));
     typedef short s16x8 __attribute__((ext_vector_type(8)));
     const s16x8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(Frag<T>, v);
@@ -189,10 +188,11 @@ DEV void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 struct KeyBits {
     const uint8_t* mask;
     int S;
-    uint8_t byte;
+    uint32_t byte;
     DEV void load(int k0, int lane) { byte = mask ? mask[min(k0 + lane, S - 1)] : 1; }
-    DEV uint64_t bits(int k0) const {
+    DEV uint64_t bits(int k0) {
         const uint64_t in = bits_below(S - k0);
+        asm volatile("" : "+v"(byte));         // (compared here and not at the load, which would wait for it there)
         return mask ? __ballot(byte != 0) & in : in;
     }
 };
@@ -234,7 +234,8 @@ constexpr float RISE = 6.0f;
 template <class T, int D>
 __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
     constexpr int ND = D / 32;
-    __shared__ u32x4 lk[2][TILE * D / 8], lv[2][TILE * D / 8];
+    constexpr int N = TILE * D / 8;
+    __shared__ u32x4 lk0[N], lk1[N], lv0[N], lv1[N];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int nq = (p.S + 127) / 128, id = xcd_order(blockIdx.x, gridDim.x);
     const int b = id / (nq * p.H), h = id / nq % p.H, i00 = id % nq * 128, i0 = i00 + 32 * wave;
@@ -256,11 +257,11 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
     const Copy<D, TILE> copy;
     KeyBits keys{p.mask ? p.mask + b * p.mask_sb : nullptr, p.S, 1};
     int k0 = tiles.at(0) * TILE;
-    copy(kp, p.k_ss, k0, p.S - 1, lk[0], wave);
-    copy(vp, p.v_ss, k0, p.S - 1, lv[0], wave);
+    copy(kp, p.k_ss, k0, p.S - 1, lk0, wave);
+    copy(vp, p.v_ss, k0, p.S - 1, lv0, wave);
     keys.load(k0, lane);
-    for (int t = 0; t < tiles.count; ++t) {
-        u32x4 *tk = lk[t & 1], *tv = lv[t & 1];
+    // tile t from tk and tv, the next one's copies into nk and nv
+    const auto turn = [&](int t, u32x4* tk, u32x4* tv, u32x4* nk, u32x4* nv) __attribute__((always_inline)) {
         arrived();
         const uint64_t bits = keys.bits(k0);
         if (bits != ~0ull) {                   // whatever memory holds of a masked key is not used
@@ -271,22 +272,22 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
         const int now = k0;
         if (t + 1 < tiles.count) {
             k0 = tiles.at(t + 1) * TILE;
-            copy(kp, p.k_ss, k0, p.S - 1, lk[(t + 1) & 1], wave);
-            copy(vp, p.v_ss, k0, p.S - 1, lv[(t + 1) & 1], wave);
+            copy(kp, p.k_ss, k0, p.S - 1, nk, wave);
+            copy(vp, p.v_ss, k0, p.S - 1, nv, wave);
             keys.load(k0, lane);
         }
-        if (bits == 0 || none_seen(p, i0, now, now + TILE - 1)) continue;
-        const uint32_t rk = fresh(lds_at(tk) + rows_at<D>(lane)), cv = fresh(lds_at(tv) + cols_at<D>(lane));
+        if (bits == 0 || i0 >= p.S || none_seen(p, i0, now, now + TILE - 1)) return;
+        const uint32_t ra = fresh(rows_at<D>(lane)), ca = fresh(cols_at<D>(lane));
         f32x16 s[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            s[u] = mfma(rows_frag<T, D>(rk, 32 * u, 0), q[0], f32x16{});
+            s[u] = mfma(rows_frag<T, D>(tk, ra, 32 * u, 0), q[0], f32x16{});
 #pragma unroll
-            for (int k = 1; k < D / 16; ++k) s[u] = mfma(rows_frag<T, D>(rk, 32 * u, k), q[k], s[u]);
+            for (int k = 1; k < D / 16; ++k) s[u] = mfma(rows_frag<T, D>(tk, ra, 32 * u, k), q[k], s[u]);
         }
         Frag<T> early[ND];                     // the first values, read while the exponentials are formed
 #pragma unroll
-        for (int d = 0; d < ND; ++d) early[d] = cols_frag<T, D>(cv, 0, d);
+        for (int d = 0; d < ND; ++d) early[d] = cols_frag<T, D>(tv, ca, 0, d);
         if (bits != ~0ull || !all_seen(p, i0, now, now + TILE - 1)) {
             const uint64_t vis = bits & bits_below(i + p.right + 1 - now) & (bits_from(i - p.left - now) | bits_below(p.sinks - now));
 #pragma unroll
@@ -330,8 +331,12 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
         for (int u = 0; u < 4; ++u) {
             const Frag<T> w = round_frag<T>(s[u / 2], u % 2);
 #pragma unroll
-            for (int d = 0; d < ND; ++d) acc[d] = mfma(u == 0 ? early[d] : cols_frag<T, D>(cv, 16 * u, d), w, acc[d]);
+            for (int d = 0; d < ND; ++d) acc[d] = mfma(u == 0 ? early[d] : cols_frag<T, D>(tv, ca, 16 * u, d), w, acc[d]);
         }
+    };
+    for (int t = 0; t < tiles.count; t += 2) {
+        turn(t, lk0, lv0, lk1, lv1);
+        if (t + 1 < tiles.count) turn(t + 1, lk1, lv1, lk0, lv0);
     }
     float l0, l1;
     swap32(l, l0, l1);
@@ -362,20 +367,12 @@ __global__ __launch_bounds__(NT) void k_attn_delta(D8sAttnArgs p, float* delta) 
     if (d == 0 && i < p.S) delta[((int64_t)b * p.H + h) * p.S + i] = x;
 }
 
-// A tile's LDS: two buffers of two tiles of 64 rows, and of a float and another for each row
-template <int D>
-struct Shared {
-    u32x4 a[2][TILE * D / 8], b[2][TILE * D / 8];
-    float e[2][TILE], d[2][TILE];
-};
-
 // Queries: as the forward pass, with do beside q: P from lse, dP = do v^T transposed, dS, dq += dS k.
 DEV float lse2_of(float lse) { return lse == -INFINITY ? INFINITY : lse * LOG2E; }   // (empty row: every P is 0)
 
 template <class T, int D>
-DEV void dq_body(const D8sAttnArgs& p, const float* delta, int id, Shared<D>& lds) {
+DEV void dq_body(const D8sAttnArgs& p, const float* delta, int id, u32x4* lk0, u32x4* lk1, u32x4* lv0, u32x4* lv1) {
     constexpr int ND = D / 32;
-    auto &lk = lds.a, &lv = lds.b;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int nq = (p.S + 127) / 128;
     const int b = id / (nq * p.H), h = id / nq % p.H, i00 = id % nq * 128, i0 = i00 + 32 * wave;
@@ -402,11 +399,11 @@ DEV void dq_body(const D8sAttnArgs& p, const float* delta, int id, Shared<D>& ld
     const Copy<D, TILE> copy;
     KeyBits keys{p.mask ? p.mask + b * p.mask_sb : nullptr, p.S, 1};
     int k0 = tiles.at(0) * TILE;
-    copy(kp, p.k_ss, k0, p.S - 1, lk[0], wave);
-    copy(vp, p.v_ss, k0, p.S - 1, lv[0], wave);
+    copy(kp, p.k_ss, k0, p.S - 1, lk0, wave);
+    copy(vp, p.v_ss, k0, p.S - 1, lv0, wave);
     keys.load(k0, lane);
-    for (int t = 0; t < tiles.count; ++t) {
-        u32x4 *tk = lk[t & 1], *tv = lv[t & 1];
+    // tile t from tk and tv, the next one's copies into nk and nv
+    const auto turn = [&](int t, u32x4* tk, u32x4* tv, u32x4* nk, u32x4* nv) __attribute__((always_inline)) {
         arrived();
         const uint64_t bits = keys.bits(k0);
         if (bits != ~0ull) {
@@ -417,23 +414,22 @@ DEV void dq_body(const D8sAttnArgs& p, const float* delta, int id, Shared<D>& ld
         const int now = k0;
         if (t + 1 < tiles.count) {
             k0 = tiles.at(t + 1) * TILE;
-            copy(kp, p.k_ss, k0, p.S - 1, lk[(t + 1) & 1], wave);
-            copy(vp, p.v_ss, k0, p.S - 1, lv[(t + 1) & 1], wave);
+            copy(kp, p.k_ss, k0, p.S - 1, nk, wave);
+            copy(vp, p.v_ss, k0, p.S - 1, nv, wave);
             keys.load(k0, lane);
         }
-        if (bits == 0 || none_seen(p, i0, now, now + TILE - 1)) continue;
-        const uint32_t rk = fresh(lds_at(tk) + rows_at<D>(lane)), rv = fresh(lds_at(tv) + rows_at<D>(lane));
-        const uint32_t ck = fresh(lds_at(tk) + cols_at<D>(lane));
+        if (bits == 0 || i0 >= p.S || none_seen(p, i0, now, now + TILE - 1)) return;
+        const uint32_t ra = fresh(rows_at<D>(lane)), ca = fresh(cols_at<D>(lane));
         const bool part = bits != ~0ull || !all_seen(p, i0, now, now + TILE - 1);
         const uint64_t vis = bits & bits_below(i + p.right + 1 - now) & (bits_from(i - p.left - now) | bits_below(p.sinks - now));
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            f32x16 s = mfma(rows_frag<T, D>(rk, 32 * u, 0), q[0], f32x16{});
-            f32x16 dp = mfma(rows_frag<T, D>(rv, 32 * u, 0), g[0], f32x16{});
+            f32x16 s = mfma(rows_frag<T, D>(tk, ra, 32 * u, 0), q[0], f32x16{});
+            f32x16 dp = mfma(rows_frag<T, D>(tv, ra, 32 * u, 0), g[0], f32x16{});
 #pragma unroll
             for (int k = 1; k < D / 16; ++k) {
-                s = mfma(rows_frag<T, D>(rk, 32 * u, k), q[k], s);
-                dp = mfma(rows_frag<T, D>(rv, 32 * u, k), g[k], dp);
+                s = mfma(rows_frag<T, D>(tk, ra, 32 * u, k), q[k], s);
+                dp = mfma(rows_frag<T, D>(tv, ra, 32 * u, k), g[k], dp);
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = exp2_(__builtin_fmaf(s[r], c, -lse2)) * (dp[r] - dl);
@@ -447,9 +443,13 @@ DEV void dq_body(const D8sAttnArgs& p, const float* delta, int id, Shared<D>& ld
                 const Frag<T> ds = round_frag<T>(s, w);
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
-                    acc[d] = mfma(cols_frag<T, D>(ck, 32 * u + 16 * w, d), ds, acc[d]);
+                    acc[d] = mfma(cols_frag<T, D>(tk, ca, 32 * u + 16 * w, d), ds, acc[d]);
             }
         }
+    };
+    for (int t = 0; t < tiles.count; t += 2) {
+        turn(t, lk0, lv0, lk1, lv1);
+        if (t + 1 < tiles.count) turn(t + 1, lk1, lv1, lk0, lv0);
     }
     store_rows<T, ND>((T*)p.dq + (((int64_t)b * p.S + i) * p.H + h) * D, acc, p.scale, i < p.S, lane);
 }
@@ -463,12 +463,15 @@ struct KeySplit {
     int sink_tiles, sink_split, split;
 };
 constexpr int KEYS = 128;
+// Operands of v that lie in LDS, each lane's own, and are read again for every product: with all of k, v, dk and dv in
+// registers some would be spilled, and a read back from scratch memory waits for the copies in flight before it
+// (dk and dv of 2 x 8199 tokens of 16 heads and their dq: 580 -> 440 us).
+constexpr int PARKED = 3;
 
 template <class T, int D>
-DEV void dkv_body(const D8sAttnArgs& p, const float* delta, float* part, KeySplit ks, int id, Shared<D>& lds) {
+DEV void dkv_body(const D8sAttnArgs& p, const float* delta, float* part, KeySplit ks, int id, u32x4* lq0, u32x4* lq1, u32x4* lg0,
+                  u32x4* lg1, float (*ls)[2 * TILE], u32x4* parked) {
     constexpr int ND = D / 32;
-    auto &lq = lds.a, &lg = lds.b;
-    auto &ls = lds.e, &ld = lds.d;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int nk = (p.S + KEYS - 1) / KEYS, G = p.H / p.HK;
     const int items = ks.sink_tiles * ks.sink_split + (nk - ks.sink_tiles) * ks.split;
@@ -490,6 +493,9 @@ DEV void dkv_body(const D8sAttnArgs& p, const float* delta, float* part, KeySpli
             v[u] = __builtin_bit_cast(Frag<T>, *(const Raw*)(vp + 16 * u));
         }
     }
+    parked += threadIdx.x;
+#pragma unroll
+    for (int x = 0; x < PARKED; ++x) parked[x * NT] = __builtin_bit_cast(u32x4, v[x]);
     // queries that see any of the keys: from j0 - right, to left past the last key or the end for a first token
     const int lo = max(0, j0 - p.right) / TILE;
     const int hi = (j0 < p.sinks ? p.S - 1 : min(p.S - 1, j0 + KEYS - 1 + p.left)) / TILE;
@@ -498,26 +504,30 @@ DEV void dkv_body(const D8sAttnArgs& p, const float* delta, float* part, KeySpli
     const float c = p.scale * LOG2E, c1 = 1.0f / p.scale;
     f32x16 dk[ND] = {}, dv[ND] = {};
     const Copy<D, TILE> copy;
-    float se = 0.0f, sd = 0.0f;
+    float se = 0.0f, sd = 0.0f;                // as they come from memory: used a turn later
+    int si = 0;
     int h = hk * G + t0 / per, qt = lo + t0 % per;         // of the tile whose copies are on their way
-    const auto load = [&](int buf) __attribute__((always_inline)) {
-        copy((const uint16_t*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, qt * TILE, p.S - 1, lq[buf], wave);
-        copy((const uint16_t*)p.dout + b * p.do_sb + h * p.do_sh, p.do_ss, qt * TILE, p.S - 1, lg[buf], wave);
+    const auto load = [&](u32x4* nq, u32x4* ng) __attribute__((always_inline)) {
+        copy((const uint16_t*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, qt * TILE, p.S - 1, nq, wave);
+        copy((const uint16_t*)p.dout + b * p.do_sb + h * p.do_sh, p.do_ss, qt * TILE, p.S - 1, ng, wave);
         if (threadIdx.x < TILE) {
             const int i = qt * TILE + threadIdx.x;
             const int64_t at = ((int64_t)b * p.H + h) * p.S + min(i, p.S - 1);
-            const float e = p.lse[at];         // (a row past the end, or that sees nothing: every P is 0)
-            se = i < p.S && e != -INFINITY ? -e * c1 : -INFINITY;
-            sd = -delta[at];
+            se = p.lse[at];
+            sd = delta[at];
+            si = i;
         }
     };
-    if (t0 < t1) load(0);
-    for (int t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1, qn = qt * TILE;
+    if (t0 < t1) load(lq0, lg0);
+    // tile t from tq and tg, its -lse / scale and -rowsum(do o) in `stats`, the next one's copies into nq and ng
+    const auto turn = [&](int t, const u32x4* tq, const u32x4* tg, float* stats, u32x4* nq, u32x4* ng) __attribute__((always_inline)) {
+        const int qn = qt * TILE;
         arrived();
         if (threadIdx.x < TILE) {
-            ls[buf][threadIdx.x] = se;
-            ld[buf][threadIdx.x] = sd;
+            asm volatile("" : "+v"(se), "+v"(sd));
+            // (a row past the end, or that sees nothing: every P is 0)
+            stats[threadIdx.x] = si < p.S && se != -INFINITY ? -se * c1 : -INFINITY;
+            stats[TILE + threadIdx.x] = -sd;
         }
         __syncthreads();                       // the tile is there, and the other one is no longer read
         if (t + 1 < t1) {
@@ -525,11 +535,10 @@ DEV void dkv_body(const D8sAttnArgs& p, const float* delta, float* part, KeySpli
                 qt = lo;
                 ++h;
             }
-            load(buf ^ 1);
+            load(nq, ng);
         }
-        if (!any) continue;
-        const uint32_t rq = fresh(lds_at(lq[buf]) + rows_at<D>(lane)), rg = fresh(lds_at(lg[buf]) + rows_at<D>(lane));
-        const uint32_t cq = fresh(lds_at(lq[buf]) + cols_at<D>(lane)), cg = fresh(lds_at(lg[buf]) + cols_at<D>(lane));
+        if (!any) return;
+        const uint32_t ra = fresh(rows_at<D>(lane)), ca = fresh(cols_at<D>(lane));
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int q0 = qn + 32 * u;
@@ -537,8 +546,8 @@ DEV void dkv_body(const D8sAttnArgs& p, const float* delta, float* part, KeySpli
             f32x16 s, dp;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const f32x4 e = *(const f32x4*)&ls[buf][32 * u + 8 * g + 4 * (lane / 32)];
-                const f32x4 d = *(const f32x4*)&ld[buf][32 * u + 8 * g + 4 * (lane / 32)];
+                const f32x4 e = *(const f32x4*)&stats[32 * u + 8 * g + 4 * (lane / 32)];
+                const f32x4 d = *(const f32x4*)&stats[TILE + 32 * u + 8 * g + 4 * (lane / 32)];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     s[4 * g + r] = e[r];
@@ -547,8 +556,8 @@ DEV void dkv_body(const D8sAttnArgs& p, const float* delta, float* part, KeySpli
             }
 #pragma unroll
             for (int x = 0; x < D / 16; ++x) {
-                s = mfma(rows_frag<T, D>(rq, 32 * u, x), k[x], s);
-                dp = mfma(rows_frag<T, D>(rg, 32 * u, x), v[x], dp);
+                s = mfma(rows_frag<T, D>(tq, ra, 32 * u, x), k[x], s);
+                dp = mfma(rows_frag<T, D>(tg, ra, 32 * u, x), x < PARKED ? __builtin_bit_cast(Frag<T>, parked[fresh(x * NT)]) : v[x], dp);
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -571,11 +580,15 @@ DEV void dkv_body(const D8sAttnArgs& p, const float* delta, float* part, KeySpli
                 const Frag<T> pf = round_frag<T>(s, w), df = round_frag<T>(dp, w);
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    dv[d] = mfma(cols_frag<T, D>(cg, 32 * u + 16 * w, d), pf, dv[d]);
-                    dk[d] = mfma(cols_frag<T, D>(cq, 32 * u + 16 * w, d), df, dk[d]);
+                    dv[d] = mfma(cols_frag<T, D>(tg, ca, 32 * u + 16 * w, d), pf, dv[d]);
+                    dk[d] = mfma(cols_frag<T, D>(tq, ca, 32 * u + 16 * w, d), df, dk[d]);
                 }
             }
         }
+    };
+    for (int t = t0; t < t1; t += 2) {
+        turn(t, lq0, lg0, ls[0], lq1, lg1);
+        if (t + 1 < t1) turn(t + 1, lq1, lg1, ls[1], lq0, lg0);
     }
     if (!on) {                                 // a masked key's column may hold anything: it has no gradient
 #pragma unroll
@@ -608,10 +621,13 @@ DEV void dkv_body(const D8sAttnArgs& p, const float* delta, float* part, KeySpli
 template <class T, int D>
 __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn_back(D8sAttnArgs p, const float* delta, float* part, KeySplit ks,
                                                                      int of_keys) {
-    __shared__ Shared<D> lds;
+    constexpr int N = TILE * D / 8;
+    __shared__ u32x4 a0[N], a1[N], b0[N], b1[N];
+    __shared__ float stats[2][2 * TILE];
+    __shared__ u32x4 parked[PARKED * NT];
     const int w = blockIdx.x;
-    if (w < of_keys) dkv_body<T, D>(p, delta, part, ks, xcd_order(w, of_keys), lds);
-    else dq_body<T, D>(p, delta, xcd_order(w - of_keys, gridDim.x - of_keys), lds);
+    if (w < of_keys) dkv_body<T, D>(p, delta, part, ks, xcd_order(w, of_keys), a0, a1, b0, b1, stats, parked);
+    else dq_body<T, D>(p, delta, xcd_order(w - of_keys, gridDim.x - of_keys), a0, a1, b0, b1);
 }
 
 // dk and dv of the split tiles: the float32 parts summed in order, four values a thread
