@@ -3,5 +3,6 @@ interface).  The directory name is not a Python identifier: load it as `rsna_kne
 `load_package()` of `__graft_entry__.py` (tests/conftest.py and bench.py do).
 
 Modules: `hip` (ctypes binding of libd8s_hip.so), `dense8s` (calibration, plan, tables, package,
-runner), `densenet` (the float DenseNet169 the plan is built from), `build` (hipcc build).
+runner), `densenet` (the float DenseNet169 the plan is built from), `build` (hipcc build); `context`, `optim` and
+`context_layer` (a context layer over all the tokens of a study, its operators and its optimizer).
 """

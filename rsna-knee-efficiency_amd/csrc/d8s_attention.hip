@@ -224,6 +224,11 @@ DEV void store_rows(T* o, const f32x16* acc, float scale, bool on, int lane) {
 }
 
 // ---- forward --------------------------------------------------------------------------------------
+// Bound by its instructions: a wave's tile of 32 x 64 scores is 162 vector operations (32 exponentials among them) beside 16
+// (D = 64) or 32 (D = 128) products of 32 cycles, and the two overlap only between waves.  Measured: 22528 tokens of 4
+// heads of 64, 1024 neighbours each, 43 us (0.41 PFLOP/s; with 32 heads 0.71 of the vector unit's time); 2 x 8199
+// tokens of 16 heads of 128, 1024 before each, 185 us (0.70 PFLOP/s).  Tiles of 32 keys and more waves: 49 and 216 us.
+//
 // A workgroup runs 128 queries of a head, 32 a wave, over the tiles of 64 keys they can see; keys and values go
 // through two LDS buffers, the next tile's copies in flight while one is computed.  A wave forms s transposed (keys x
 // queries), so a query's statistics are one value a lane, and P goes from registers into the second product.
@@ -349,8 +354,10 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
 // ---- backward ----------------------------------------------------------------------------------------
 // k_attn_delta leaves rowsum(do o) of every query.  One launch then runs both kinds of workgroups beside each other:
 // first those of the keys (dk and dv, the longer ones), then those of the queries (dq), which fill the compute units
-// that the keys leave; what either writes the other does not read.  Both form s and dP again: a third product more
+// that the keys leave; what either writes the other does not read.  Both form s and dP: two products of seven more
 // than sums shared through atomics would take, for results that do not depend on an order.
+// Bound as the forward pass, with the matrix unit busy 0.48 of the time: 2 x 8199 tokens of 16 heads of 128 (4 key heads),
+// 1024 before each, in 530 .. 560 us (0.6 PFLOP/s with the products formed twice); one launch after the other 690.
 template <class T, int D>
 __global__ __launch_bounds__(NT) void k_attn_delta(D8sAttnArgs p, float* delta) {
     constexpr int L = D / 8, ROWS = NT / L;    // lanes a row, rows a workgroup
@@ -464,8 +471,8 @@ struct KeySplit {
 };
 constexpr int KEYS = 128;
 // Operands of v that lie in LDS, each lane's own, and are read again for every product: with all of k, v, dk and dv in
-// registers some would be spilled, and a read back from scratch memory waits for the copies in flight before it
-// (dk and dv of 2 x 8199 tokens of 16 heads and their dq: 580 -> 440 us).
+// registers nine of a lane's are spilled at D = 128, and a read back from scratch memory waits for the copies in
+// flight before it.
 constexpr int PARKED = 3;
 
 template <class T, int D>
@@ -677,7 +684,8 @@ uint64_t delta_bytes(const D8sAttnArgs* a) { return ((uint64_t)a->B * a->H * a->
 // A workgroup runs GM query heads of a key head over a share of the keys their token sees.  A key's row is read 16
 // bytes a lane by D / 8 lanes, so a wave reads 8 (D = 64) or 4 rows at a time; each group of lanes keeps the softmax
 // statistics and the sums of its own keys, and they are joined at the end, across the groups, the waves, and (k_join)
-// the shares.  Bound by memory: every key and value is read once for all the heads that share it (up to 8).
+// the shares.  Bound by memory: every key and value is read once for all the heads that share it (up to 8).  Measured:
+// 64 requests of 1 .. 8192 tokens, 4096 visible, 32 heads on 8 key heads of 128: 170 us (4.7 TB/s).
 template <class T, int D, int GM>
 __global__ __launch_bounds__(NT) void k_token(D8sTokenArgs p, int split, float* part) {
     constexpr int LK = D / 8, KW = 64 / LK, U = 4;
@@ -830,9 +838,9 @@ __global__ __launch_bounds__(NT) void k_join(const float* part, T* out, int spli
     out[(int64_t)head * D + d] = (T)(sum > 0.0f || sum != sum ? o / sum : 0.0f);
 }
 
-// Shares of a token's keys: enough workgroups for `TOKEN_WGS` a compute unit, at least the keys of one turn of a
-// workgroup's waves each
-constexpr int TOKEN_WGS = 4;
+// Shares of a token's keys: enough workgroups for TOKEN_WGS a compute unit, so that long and short rows even out (the 64
+// requests above: 170 us; with 8 a compute unit 176, with 4 186), at least the keys of one turn of a workgroup's waves each
+constexpr int TOKEN_WGS = 16;
 int token_split(const D8sTokenArgs* a) {
     const int G = a->H / a->HK, gm = G > 4 ? 8 : G > 2 ? 4 : G;
     const int64_t problems = (int64_t)a->B * a->HK * ((G + gm - 1) / gm);

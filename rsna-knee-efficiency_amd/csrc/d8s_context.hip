@@ -6,7 +6,9 @@
 //   g = dy w,  dx = r (g - mean g - xh mean(g xh)),  dw = sum over rows of dy xh,  db = sum over rows of dy.
 // All sums are float32; the variance is of the centred values (a second look at the registers), so a large mean
 // costs no digits.  Bound by memory: a row is read once into the registers of the 16 lanes, the wave or the
-// workgroup it is shared between, everything else happens there, and it is written once.
+// workgroup it is shared between, everything else happens there, and it is written once.  Measured, 98303 rows of 1024
+// bfloat16: forward 81 us (5.0 TB/s; a large copy on this card 5.2), gradients 110 us (5.5 TB/s) and 8 us for the
+// columns' sums.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -224,6 +226,8 @@ __global__ __launch_bounds__(256) void k_norm_cols(D8sNormArgs p, int parts) {
 // Rows per workgroup of the shape that runs `width`
 int norm_rows(int width) { return width <= 128 ? 16 : width <= 2048 ? 4 : 1; }
 
+// Workgroups of the gradients, each of which leaves a part of the columns' sums: four a compute unit keep enough rows
+// in flight (98303 x 1024 bfloat16: 113 us; two a compute unit 165 us, and 4 us less for the sums)
 int norm_parts(const D8sNormArgs* a) {
     const int64_t per = norm_rows(a->width), all = (a->rows + per - 1) / per;
     return (int)std::min<int64_t>(all, 4 * d8s_host_cu_count());
@@ -280,7 +284,7 @@ int norm_check(const D8sNormArgs* a, const char* what) {
 // which is also the gradient, turns back.  The angle is formed in float64 as a number of turns and its whole turns
 // dropped there (three operations), so any position an int32 holds is as exact as a small one; sine and cosine of
 // the rest are float32.  A thread forms those of V pairs of a token once and applies them to the token's heads.
-// Bound by memory.
+// Bound by memory: 49152 tokens of 20 heads of 128 float16 channels in 101 us (5.0 TB/s).
 template <class T, bool ADJ>
 __global__ __launch_bounds__(256) void k_rotary(D8sRotaryArgs p, int groups, int turned, int per) {
     constexpr int V = 16 / (int)sizeof(T);
@@ -351,7 +355,7 @@ void rotary_run(const D8sRotaryArgs& a, hipStream_t st) {
     const int groups = turned + (rest + 2 * V - 1) / (2 * V);
     const int64_t threads = (int64_t)a.B * a.S * groups, blocks = (threads + 255) / 256;
     // heads a thread: all of them share its sines and cosines, unless that leaves fewer than 8 waves a compute unit
-    // (28 us of latency, not memory, for 8 heads of 7128 tokens)
+    // (8 heads of 7128 tokens: 10.8 us with all heads a thread, 8.4 with two)
     const int64_t want = 8 * 64 * (int64_t)d8s_host_cu_count();
     const int ys = (int)std::min<int64_t>(a.H, std::max<int64_t>(1, want / std::max<int64_t>(1, threads)));
     const int per = (a.H + ys - 1) / ys;
