@@ -167,6 +167,8 @@ def _rotate(x, positions, sections, base, adjacent, inverse, out):
         out = _like(x)
     elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(3) != 1:
         _fail("out must be like x, its channels contiguous")
+    elif out.data_ptr() == x.data_ptr() and out.stride() != x.stride():
+        _fail("out must be x itself, or memory of its own")
     if not x.numel():
         return out
     a.x, a.y, a.pos = x.data_ptr(), out.data_ptr(), positions.data_ptr()

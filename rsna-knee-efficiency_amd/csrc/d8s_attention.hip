@@ -297,6 +297,7 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
             const uint64_t vis = bits & bits_below(i + p.right + 1 - now) & (bits_from(i - p.left - now) | bits_below(p.sinks - now));
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
+                if ((uint32_t)(bits >> (32 * u)) == ~0u && all_seen(p, i0, now + 32 * u, now + 32 * u + 31)) continue;
                 const uint32_t mine = lane_rows((uint32_t)(vis >> (32 * u)), lane);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
@@ -427,10 +428,10 @@ DEV void dq_body(const D8sAttnArgs& p, const float* delta, int id, u32x4* lk0, u
         }
         if (bits == 0 || i0 >= p.S || none_seen(p, i0, now, now + TILE - 1)) return;
         const uint32_t ra = fresh(rows_at<D>(lane)), ca = fresh(cols_at<D>(lane));
-        const bool part = bits != ~0ull || !all_seen(p, i0, now, now + TILE - 1);
         const uint64_t vis = bits & bits_below(i + p.right + 1 - now) & (bits_from(i - p.left - now) | bits_below(p.sinks - now));
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
+            if ((uint32_t)(bits >> (32 * u)) == 0 || none_seen(p, i0, now + 32 * u, now + 32 * u + 31)) continue;
             f32x16 s = mfma(rows_frag<T, D>(tk, ra, 32 * u, 0), q[0], f32x16{});
             f32x16 dp = mfma(rows_frag<T, D>(tv, ra, 32 * u, 0), g[0], f32x16{});
 #pragma unroll
@@ -440,7 +441,7 @@ DEV void dq_body(const D8sAttnArgs& p, const float* delta, int id, u32x4* lk0, u
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = exp2_(__builtin_fmaf(s[r], c, -lse2)) * (dp[r] - dl);
-            if (part) {
+            if ((uint32_t)(bits >> (32 * u)) != ~0u || !all_seen(p, i0, now + 32 * u, now + 32 * u + 31)) {
                 const uint32_t mine = lane_rows((uint32_t)(vis >> (32 * u)), lane);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = __uint_as_float(__float_as_uint(s[r]) & keep_mask(mine, r));

@@ -231,3 +231,6 @@ def test_rotary_strides_in_place_and_gradient(dev):
     assert context.rotary(x.detach()[:, :0], pos[:, :0], (8, 12, 12)).shape == (2, 0, 4, 64)
     with pytest.raises(ValueError, match="out"):
         context.rotary(x, pos, (8, 12, 12), out=torch.empty_like(x))
+    square = torch.randn((4, 4, 1, 8), generator=g, device=dev)
+    with pytest.raises(ValueError, match="memory of its own"):
+        context.rotary(square, pos[0, :4, :1], (4,), out=square.transpose(0, 1))
