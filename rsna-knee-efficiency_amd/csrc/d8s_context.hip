@@ -31,11 +31,37 @@ using namespace d8s;
 constexpr int NORM_MAX = 16384;
 
 // ---- layer norm -----------------------------------------------------------------------------------
-// TPR threads share a row, each holding E of its values in vectors of V (16 bytes): vector v of thread t holds
-// columns (v TPR + t) V ...
+// TPR threads share a row, each holding E of its values in vectors of V (16 bytes): vector v of thread t holds columns
+// (v TPR + t) V ...  A row's last vector, where V does not divide the width, is read value by value, which in short rows
+// costs up to half of the time.  There (WHOLE: eight values a thread) it ends with the row instead: its first `again`
+// values are the ones before it once more, are left out of sums, and what is computed of them is the same bits as the
+// other thread's, and both store it.  60000 rows of 300 bfloat16: forward 30 -> 25 us, gradients 57 -> 36; with more values
+// a thread the sums' second form costs registers, and more than it gives (10000 rows of 2000: 53 -> 71 us).
+struct Place {
+    int c, n, again;                           // first column, columns from it to the row's end (0: none), and see above
+};
+template <int V, bool WHOLE>
+DEV Place place(int vector, int width) {
+    const int c = vector * V;
+    if (c >= width) return {0, 0, 0};
+    const int at = WHOLE && width >= V ? min(c, width - V) : c;
+    return {at, width - at, c - at};
+}
+// The vector's own values, zeros in place of the others (whose bits may be anything)
+template <int V>
+DEV void only_own(const Place& at, const float* f, float* own) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) own[i] = f[i];
+    if (at.again != 0 || at.n < V) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) own[i] = i >= at.again && i < at.n ? f[i] : 0.0f;
+    }
+}
+
 template <class T, int TPR, int E>
 struct NormShape {
     static constexpr int V = 16 / (int)sizeof(T), NV = E / V;
+    static constexpr bool WHOLE = E == 8;
     static constexpr int THREADS = TPR > 256 ? TPR : 256, RPW = THREADS / TPR, WAVES = THREADS / 64;
     static_assert(E % V == 0, "whole vectors");
 };
@@ -77,22 +103,32 @@ __global__ __launch_bounds__((NormShape<T, TPR, E>::THREADS)) void k_norm(D8sNor
         float sum = 0.0f, zero = 0.0f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int c = (v * TPR + t) * V;
-            load_n<T, V>(x + c, on ? p.width - c : 0, f + v * V);
+            const Place at = place<V, S::WHOLE>(v * TPR + t, p.width);
+            load_n<T, V>(x + at.c, on ? at.n : 0, f + v * V);
         }
 #pragma unroll
-        for (int i = 0; i < E; ++i) sum += f[i];
+        for (int v = 0; v < NV; ++v) {
+            float own[V];
+            if constexpr (S::WHOLE) only_own<V>(place<V, true>(v * TPR + t, p.width), f + v * V, own);
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum += S::WHOLE ? own[i] : f[v * V + i];
+        }
         row_sum2<TPR, S::WAVES>(sum, zero, red);
         const float mean = sum / (float)p.width;
         float sq = 0.0f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int n = p.width - (v * TPR + t) * V;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                float d = f[v * V + i] - mean;
-                f[v * V + i] = d;
-                sq = i < n ? __builtin_fmaf(d, d, sq) : sq;
+            for (int i = 0; i < V; ++i) f[v * V + i] -= mean;
+            if constexpr (S::WHOLE) {
+                float own[V];
+                only_own<V>(place<V, true>(v * TPR + t, p.width), f + v * V, own);
+#pragma unroll
+                for (int i = 0; i < V; ++i) sq = __builtin_fmaf(own[i], own[i], sq);
+            } else {
+                const int n = p.width - (v * TPR + t) * V;
+#pragma unroll
+                for (int i = 0; i < V; ++i) sq = i < n ? __builtin_fmaf(f[v * V + i], f[v * V + i], sq) : sq;
             }
         }
         row_sum2<TPR, S::WAVES>(sq, zero, red);
@@ -105,14 +141,14 @@ __global__ __launch_bounds__((NormShape<T, TPR, E>::THREADS)) void k_norm(D8sNor
         T* y = (T*)p.y + r * p.width;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int c = (v * TPR + t) * V, n = p.width - c;
-            if (n <= 0) continue;
+            const Place at = place<V, S::WHOLE>(v * TPR + t, p.width);
+            if (at.n == 0) continue;
             float w[V], b[V], o[V];
-            load_n<W, V>((const W*)p.w + c, n, w);
-            if (p.b) load_n<W, V>((const W*)p.b + c, n, b);
+            load_n<W, V>((const W*)p.w + at.c, at.n, w);
+            if (p.b) load_n<W, V>((const W*)p.b + at.c, at.n, b);
 #pragma unroll
             for (int i = 0; i < V; ++i) o[i] = __builtin_fmaf(f[v * V + i] * rstd, w[i], p.b ? b[i] : 0.0f);
-            store_n<T, V>(y + c, n, o);
+            store_n<T, V>(y + at.c, at.n, o);
         }
     }
 }
@@ -129,8 +165,8 @@ __global__ __launch_bounds__((NormShape<T, TPR, E>::THREADS)) void k_norm_back(D
     float w[E], dw[E], db[E];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        const int c = (v * TPR + t) * V;
-        load_n<W, V>((const W*)p.w + c, p.width - c, w + v * V);
+        const Place at = place<V, S::WHOLE>(v * TPR + t, p.width);
+        load_n<W, V>((const W*)p.w + at.c, at.n, w + v * V);
     }
 #pragma unroll
     for (int i = 0; i < E; ++i) dw[i] = db[i] = 0.0f;
@@ -144,20 +180,34 @@ __global__ __launch_bounds__((NormShape<T, TPR, E>::THREADS)) void k_norm_back(D
         float f[E], g[E];
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int c = (v * TPR + t) * V, n = on ? p.width - c : 0;
-            load_n<T, V>(x + c, n, f + v * V);
-            load_n<T, V>(dy + c, n, g + v * V);
+            const Place at = place<V, S::WHOLE>(v * TPR + t, p.width);
+            const int n = on ? at.n : 0;
+            load_n<T, V>(x + at.c, n, f + v * V);
+            load_n<T, V>(dy + at.c, n, g + v * V);
         }
         float s1 = 0.0f, s2 = 0.0f;
-        // (past the row's end dy and w are zeros: nothing is added)
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             f[i] = (f[i] - mean) * rstd;
             dw[i] = __builtin_fmaf(g[i], f[i], dw[i]);
             db[i] += g[i];
             g[i] *= w[i];
-            s1 += g[i];
-            s2 = __builtin_fmaf(g[i], f[i], s2);
+            if constexpr (!S::WHOLE) {         // (past the row's end dy and w are zeros: nothing is added)
+                s1 += g[i];
+                s2 = __builtin_fmaf(g[i], f[i], s2);
+            }
+        }
+        if constexpr (S::WHOLE) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                float own[V];
+                only_own<V>(place<V, true>(v * TPR + t, p.width), g + v * V, own);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    s1 += own[i];
+                    s2 = __builtin_fmaf(own[i], f[v * V + i], s2);
+                }
+            }
         }
         row_sum2<TPR, S::WAVES>(s1, s2, red);
         s1 *= inv;
@@ -166,13 +216,13 @@ __global__ __launch_bounds__((NormShape<T, TPR, E>::THREADS)) void k_norm_back(D
         T* dx = (T*)p.dx + r * p.width;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int c = (v * TPR + t) * V, n = p.width - c;
-            if (n <= 0) continue;
+            const Place at = place<V, S::WHOLE>(v * TPR + t, p.width);
+            if (at.n == 0) continue;
             float o[V];
 #pragma unroll
             for (int i = 0; i < V; ++i)
                 o[i] = rstd * (g[v * V + i] - __builtin_fmaf(f[v * V + i], s2, s1));
-            store_n<T, V>(dx + c, n, o);
+            store_n<T, V>(dx + at.c, at.n, o);
         }
     }
     float* out = p.partial + (int64_t)blockIdx.x * 2 * p.width;
@@ -182,9 +232,13 @@ __global__ __launch_bounds__((NormShape<T, TPR, E>::THREADS)) void k_norm_back(D
         if constexpr (RPW > 1) {
             __syncthreads();
 #pragma unroll
-            for (int v = 0; v < NV; ++v)
+            for (int v = 0; v < NV; ++v) {
+                const Place at = place<V, S::WHOLE>(v * TPR + t, p.width);
 #pragma unroll
-                for (int i = 0; i < V; ++i) part[sub * TPR * E + (v * TPR + t) * V + i] = a[v * V + i];
+                for (int i = 0; i < V; ++i)
+                    if (!S::WHOLE) part[sub * TPR * E + (v * TPR + t) * V + i] = a[v * V + i];
+                    else if (i >= at.again && i < at.n) part[sub * TPR * E + at.c + i] = a[v * V + i];
+            }
             __syncthreads();
             for (int c = threadIdx.x; c < p.width; c += S::THREADS) {
                 float s = part[c];
@@ -195,8 +249,8 @@ __global__ __launch_bounds__((NormShape<T, TPR, E>::THREADS)) void k_norm_back(D
         } else {
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                const int c = (v * TPR + t) * V;
-                if (c < p.width) store_n<float, V>(out + k * p.width + c, p.width - c, a + v * V);
+                const Place at = place<V, S::WHOLE>(v * TPR + t, p.width);
+                store_n<float, V>(out + k * p.width + at.c, at.n, a + v * V);
             }
         }
     }
