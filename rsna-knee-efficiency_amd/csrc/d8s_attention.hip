@@ -103,6 +103,9 @@ DEV Frag<T> cols_frag(const u32x4* tile, uint32_t at, int r0, int d) {
     return __builtin_bit_cast(Frag<T>, v);
 }
 
+// Registers 8 s .. of a result as the next product's operand.  P and dS are rounded to T here because the matrix unit's
+// full rate takes 16-bit operands (float32 ones a sixteenth of it): 2^-9 (bf16) or 2^-12 of each value, independent from
+// value to value, about what the results' own rounding to T adds; P's sum and the statistics stay float32.
 template <class T>
 DEV Frag<T> round_frag(const f32x16& x, int s) {
     Frag<T> f;
@@ -226,8 +229,8 @@ DEV void store_rows(T* o, const f32x16* acc, float scale, bool on, int lane) {
 // ---- forward --------------------------------------------------------------------------------------
 // Bound by its instructions: a wave's tile of 32 x 64 scores is 162 vector operations (32 exponentials among them) beside 16
 // (D = 64) or 32 (D = 128) products of 32 cycles, and the two overlap only between waves.  Measured: 22528 tokens of 4
-// heads of 64, 1024 neighbours each, 43 us (0.41 PFLOP/s; with 32 heads 0.71 of the vector unit's time); 2 x 8199
-// tokens of 16 heads of 128, 1024 before each, 185 us (0.70 PFLOP/s).  Tiles of 32 keys and more waves: 49 and 216 us.
+// heads of 64, 1024 neighbours each, 43 us (0.41 PFLOP/s; 32 heads without a mask 0.68); 2 x 8199
+// tokens of 16 heads of 128, 1024 before each, 181 us (0.72 PFLOP/s).  Tiles of 32 keys and more waves: 49 and 216 us.
 //
 // A workgroup runs 128 queries of a head, 32 a wave, over the tiles of 64 keys they can see; keys and values go
 // through two LDS buffers, the next tile's copies in flight while one is computed.  A wave forms s transposed (keys x
@@ -358,7 +361,7 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
 // that the keys leave; what either writes the other does not read.  Both form s and dP: two products of seven more
 // than sums shared through atomics would take, for results that do not depend on an order.
 // Bound as the forward pass, with the matrix unit busy 0.48 of the time: 2 x 8199 tokens of 16 heads of 128 (4 key heads),
-// 1024 before each, in 530 .. 560 us (0.6 PFLOP/s with the products formed twice); one launch after the other 690.
+// 1024 before each, in 514 .. 561 us (0.6 PFLOP/s with the products formed twice; two launches after each other took 700).
 template <class T, int D>
 __global__ __launch_bounds__(NT) void k_attn_delta(D8sAttnArgs p, float* delta) {
     constexpr int L = D / 8, ROWS = NT / L;    // lanes a row, rows a workgroup
