@@ -516,7 +516,8 @@ int d8s_rotary(const D8sRotaryArgs* a, void* stream);
  * (D8S_BF16 or D8S_F16; D 64 or 128; H a multiple of HK, query head h uses key head h / (H / HK)) with the given
  * strides (elements, the last dimension contiguous); out, dq [B][S][H][D], dk, dv [B][S][HK][D] and lse [B][H][S]
  * (natural logarithm of the sum of exponentials) contiguous.  Products are of 16 bits with float32 sums; P and dS
- * are rounded to dtype between two products.  Equal inputs give equal bits.
+ * are rounded to dtype between two products (for D8S_F16 the gradients multiply both by powers of two that bring them into
+ * its range, and divide the results by them).  Equal inputs give equal bits.
  *   d8s_attention:           writes out, and lse unless 0;
  *   d8s_attention_backward:  reads out and lse beside the inputs; writes dq, dk, dv; `workspace` is device memory of
  *                            d8s_attention_workspace bytes, 16-byte aligned. */

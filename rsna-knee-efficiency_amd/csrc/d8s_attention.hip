@@ -104,8 +104,9 @@ DEV Frag<T> cols_frag(const u32x4* tile, uint32_t at, int r0, int d) {
 }
 
 // Registers 8 s .. of a result as the next product's operand.  P and dS are rounded to T here because the matrix unit's
-// full rate takes 16-bit operands (float32 ones a sixteenth of it): 2^-9 (bf16) or 2^-12 of each value, independent from
-// value to value, about what the results' own rounding to T adds; P's sum and the statistics stay float32.
+// full rate takes 16-bit operands (float32 ones a sixteenth of it): at most 2^-8 (bf16) or 2^-11 (f16, above 2^-14) of
+// each value, independent from value to value, about what the results' own rounding to T adds; P's sum and the
+// statistics stay float32.  The gradients bring P and dS into the range where that holds for f16 (see backward).
 template <class T>
 DEV Frag<T> round_frag(const f32x16& x, int s) {
     Frag<T> f;
@@ -356,33 +357,118 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
 }
 
 // ---- backward ----------------------------------------------------------------------------------------
+// float16 holds values of 2^-14 .. 2^16 in full, and dS = P (dP - rowsum(do o)) is a share of 1 / (keys seen) of a
+// gradient that may itself be small, or multiplied by a large loss scale.  So there dS is formed times a power of two,
+// which the results are divided by (exact): |dP - rowsum| <= |do||v| + |rowsum|, so from the largest |do| and |rowsum| of
+// the queries that a workgroup runs over (dk; of a lane's own query for dq) and the largest |v| of the keys follows a power
+// that keeps |dS| below 2^15 (P is 1 at most, 2 with its rounding), and nothing above 2^-28 of that bound is
+// held in fewer bits.  It is in the exponent that P is formed from (for dk partly in v), so a tile costs no operation
+// more: 2 x 8199 tokens of 16 heads of 128, 541 us with it and 535 without.  bfloat16 has float32's range and needs none.  The largest
+// norms of every tile of 64 queries and of 64 keys are left by k_attn_delta; queries that see nothing, keys that are
+// masked and rows that are not finite are left out of them, so that they do not cost the others their bits.
+//
 // k_attn_delta leaves rowsum(do o) of every query.  One launch then runs both kinds of workgroups beside each other:
 // first those of the keys (dk and dv, the longer ones), then those of the queries (dq), which fill the compute units
 // that the keys leave; what either writes the other does not read.  Both form s and dP: two products of seven more
 // than sums shared through atomics would take, for results that do not depend on an order.
 // Bound as the forward pass, with the matrix unit busy 0.48 of the time: 2 x 8199 tokens of 16 heads of 128 (4 key heads),
 // 1024 before each, in 514 .. 561 us (0.6 PFLOP/s with the products formed twice; two launches after each other took 700).
-template <class T, int D>
-__global__ __launch_bounds__(NT) void k_attn_delta(D8sAttnArgs p, float* delta) {
-    constexpr int L = D / 8, ROWS = NT / L;    // lanes a row, rows a workgroup
-    const int runs = (p.S + ROWS - 1) / ROWS;
-    const int run = blockIdx.x % runs, h = blockIdx.x / runs % p.H, b = blockIdx.x / runs / p.H;
-    const int i = run * ROWS + threadIdx.x / L, d = threadIdx.x % L * 8;
-    const int64_t ic = min(i, p.S - 1);
-    float g[8], o[8], x = 0.0f;
-    load_n<T, 8>((const T*)p.dout + b * p.do_sb + h * p.do_sh + ic * p.do_ss + d, 8, g);
-    load_n<T, 8>((const T*)p.out + (((int64_t)b * p.S + ic) * p.H + h) * D + d, 8, o);
+template <class T>
+constexpr bool NARROW = false;                 // whether P and dS are brought into T's range
+template <>
+constexpr bool NARROW<f16> = true;
+
+// Of each tile of 64 rows: the largest |do| and |rowsum(do o)| [B][H][tiles], the largest |v| [B][HK][tiles]
+struct Tops {
+    float *g, *r, *v;
+};
+DEV float wave_max(float x) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x = __builtin_fmaf(g[k], o[k], x);
-    x = lanes_sum<L>(x);
-    if (d == 0 && i < p.S) delta[((int64_t)b * p.H + h) * p.S + i] = x;
+    for (int o = 32; o >= 1; o /= 2) x = fmaxf(x, __shfl_xor(x, o));
+    return x;
+}
+// The power of two (its exponent) that brings values of at most `bound` below 2^14
+DEV int shift_of(float bound) {
+    return bound > 0.0f && bound < INFINITY ? min(max(14 - __builtin_amdgcn_frexp_expf(bound), -64), 64) : 0;
+}
+DEV float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+// The sum of squares of a row whose other half is held by the lane 32 away
+template <class T, int N>
+DEV float row_square(const Frag<T>* f) {
+    float x = 0.0f, a, b;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x = __builtin_fmaf((float)f[k][j], (float)f[k][j], x);
+    swap32(x, a, b);
+    return a + b;
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(NT) void k_attn_delta(D8sAttnArgs p, float* delta, Tops tops) {
+    constexpr int L = D / 8, ROWS = NT / L;    // lanes a row, rows at a time
+    constexpr int TURNS = NARROW<T> ? TILE / ROWS : 1;
+    const int run_rows = ROWS * TURNS, runs = (p.S + run_rows - 1) / run_rows, of_queries = p.B * p.H * runs;
+    const bool keys = NARROW<T> && (int)blockIdx.x >= of_queries;
+    const int id = keys ? blockIdx.x - of_queries : blockIdx.x, heads = keys ? p.HK : p.H;
+    const int run = id % runs, h = id / runs % heads, b = id / runs / heads, d = threadIdx.x % L * 8;
+    float first = 0.0f, second = 0.0f;         // the largest squares; rowsums
+#pragma unroll
+    for (int n = 0; n < TURNS; ++n) {
+        const int i = run * run_rows + n * ROWS + threadIdx.x / L;
+        const int64_t ic = min(i, p.S - 1);
+        if (NARROW<T> && keys) {
+            float v[8], x = 0.0f;
+            load_n<T, 8>((const T*)p.v + b * p.v_sb + h * p.v_sh + ic * p.v_ss + d, 8, v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x = __builtin_fmaf(v[k], v[k], x);
+            x = lanes_sum<L>(x);
+            const bool on = p.mask == nullptr || p.mask[b * p.mask_sb + ic] != 0;
+            first = fmaxf(first, on && x < INFINITY ? x : 0.0f);
+            continue;
+        }
+        float g[8], o[8], x = 0.0f, y = 0.0f;
+        load_n<T, 8>((const T*)p.dout + b * p.do_sb + h * p.do_sh + ic * p.do_ss + d, 8, g);
+        load_n<T, 8>((const T*)p.out + (((int64_t)b * p.S + ic) * p.H + h) * D + d, 8, o);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x = __builtin_fmaf(g[k], o[k], x);
+        x = lanes_sum<L>(x);
+        const int64_t at = ((int64_t)b * p.H + h) * p.S;
+        if (d == 0 && i < p.S) delta[at + i] = x;
+        if constexpr (NARROW<T>) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y = __builtin_fmaf(g[k], g[k], y);
+            y = lanes_sum<L>(y);
+            const bool on = p.lse[at + ic] != -INFINITY && y < INFINITY && fabsf(x) < INFINITY;
+            first = fmaxf(first, on ? y : 0.0f);
+            second = fmaxf(second, on ? fabsf(x) : 0.0f);
+        }
+    }
+    if constexpr (NARROW<T>) {
+        __shared__ float red[2][NT / 64];
+        first = wave_max(first);
+        second = wave_max(second);
+        if (threadIdx.x % 64 == 0) {
+            red[0][threadIdx.x / 64] = first;
+            red[1][threadIdx.x / 64] = second;
+        }
+        __syncthreads();
+        if (threadIdx.x != 0) return;
+#pragma unroll
+        for (int w = 1; w < NT / 64; ++w) {
+            first = fmaxf(first, red[0][w]);
+            second = fmaxf(second, red[1][w]);
+        }
+        (keys ? tops.v : tops.g)[id] = sqrtf(first);
+        if (!keys) tops.r[id] = second;
+    }
 }
 
 // Queries: as the forward pass, with do beside q: P from lse, dP = do v^T transposed, dS, dq += dS k.
 DEV float lse2_of(float lse) { return lse == -INFINITY ? INFINITY : lse * LOG2E; }   // (empty row: every P is 0)
 
 template <class T, int D>
-DEV void dq_body(const D8sAttnArgs& p, const float* delta, int id, u32x4* lk0, u32x4* lk1, u32x4* lv0, u32x4* lv1) {
+DEV void dq_body(const D8sAttnArgs& p, const float* delta, const Tops& tops, int id, u32x4* lk0, u32x4* lk1, u32x4* lv0, u32x4* lv1) {
     constexpr int ND = D / 32;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int nq = (p.S + 127) / 128;
@@ -404,7 +490,8 @@ DEV void dq_body(const D8sAttnArgs& p, const float* delta, int id, u32x4* lk0, u
         }
     }
     const int64_t stat = ((int64_t)b * p.H + h) * p.S + ic;
-    const float c = p.scale * LOG2E, lse2 = lse2_of(p.lse[stat]), dl = delta[stat];
+    const float c = p.scale * LOG2E, dl = delta[stat];
+    float lse2 = lse2_of(p.lse[stat]), unscale = p.scale;
     f32x16 acc[ND] = {};
     const Tiles tiles = tiles_of(p, i00, min(i00 + 127, p.S - 1));
     const Copy<D, TILE> copy;
@@ -414,6 +501,14 @@ DEV void dq_body(const D8sAttnArgs& p, const float* delta, int id, u32x4* lk0, u
     copy(vp, p.v_ss, k0, p.S - 1, lv0, wave);
     keys.load(k0, lane);
     // tile t from tk and tv, the next one's copies into nk and nv
+    if constexpr (NARROW<T>) {                 // P, and so dS, times a power of two of the query's own
+        const int nt = (p.S + TILE - 1) / TILE;
+        float top = 0.0f;
+        for (int t = lane; t < tiles.count; t += 64) top = fmaxf(top, tops.v[((int64_t)b * p.HK + hk) * nt + tiles.at(t)]);
+        const int e = shift_of(__builtin_fmaf(sqrtf(row_square<T, D / 16>(g)), wave_max(top), fabsf(dl)));
+        lse2 -= (float)e;
+        unscale *= power_of_two(-e);
+    }
     const auto turn = [&](int t, u32x4* tk, u32x4* tv, u32x4* nk, u32x4* nv) __attribute__((always_inline)) {
         arrived();
         const uint64_t bits = keys.bits(k0);
@@ -462,7 +557,7 @@ DEV void dq_body(const D8sAttnArgs& p, const float* delta, int id, u32x4* lk0, u
         turn(t, lk0, lv0, lk1, lv1);
         if (t + 1 < tiles.count) turn(t + 1, lk1, lv1, lk0, lv0);
     }
-    store_rows<T, ND>((T*)p.dq + (((int64_t)b * p.S + i) * p.H + h) * D, acc, p.scale, i < p.S, lane);
+    store_rows<T, ND>((T*)p.dq + (((int64_t)b * p.S + i) * p.H + h) * D, acc, unscale, i < p.S, lane);
 }
 
 // Keys: a workgroup runs 128 keys of a key head, 32 a wave, over the tiles of 64 queries that see them, one query head of
@@ -480,7 +575,7 @@ constexpr int KEYS = 128;
 constexpr int PARKED = 3;
 
 template <class T, int D>
-DEV void dkv_body(const D8sAttnArgs& p, const float* delta, float* part, KeySplit ks, int id, u32x4* lq0, u32x4* lq1, u32x4* lg0,
+DEV void dkv_body(const D8sAttnArgs& p, const float* delta, const Tops& tops, float* part, KeySplit ks, int id, u32x4* lq0, u32x4* lq1, u32x4* lg0,
                   u32x4* lg1, float (*ls)[2 * TILE], u32x4* parked) {
     constexpr int ND = D / 32;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -504,9 +599,6 @@ DEV void dkv_body(const D8sAttnArgs& p, const float* delta, float* part, KeySpli
             v[u] = __builtin_bit_cast(Frag<T>, *(const Raw*)(vp + 16 * u));
         }
     }
-    parked += threadIdx.x;
-#pragma unroll
-    for (int x = 0; x < PARKED; ++x) parked[x * NT] = __builtin_bit_cast(u32x4, v[x]);
     // queries that see any of the keys: from j0 - right, to left past the last key or the end for a first token
     const int lo = max(0, j0 - p.right) / TILE;
     const int hi = (j0 < p.sinks ? p.S - 1 : min(p.S - 1, j0 + KEYS - 1 + p.left)) / TILE;
@@ -530,15 +622,49 @@ DEV void dkv_body(const D8sAttnArgs& p, const float* delta, float* part, KeySpli
         }
     };
     if (t0 < t1) load(lq0, lg0);
-    // tile t from tq and tg, its -lse / scale and -rowsum(do o) in `stats`, the next one's copies into nq and ng
+    // The powers of two (exponents) of P and of v, which dS then has both of: P's between 0 and 14 as far as v can take the
+    // rest (raised as far as float16 goes, which costs it no bits, or lowered by 2^10 at most, which costs it what lies
+    // below 2^-15)
+    int of_p = 0, of_v = 0;
+    if constexpr (NARROW<T>) {
+        const int nt = (p.S + TILE - 1) / TILE;
+        float tops_of[3] = {};                 // |do|, |rowsum(do o)| of the queries, |v| of the keys
+        for (int t = t0 + (int)threadIdx.x; t < t1; t += NT) {
+            const int64_t at = ((int64_t)b * p.H + hk * G + t / per) * nt + lo + t % per;
+            tops_of[0] = fmaxf(tops_of[0], tops.g[at]);
+            tops_of[1] = fmaxf(tops_of[1], tops.r[at]);
+        }
+        if (threadIdx.x < KEYS / TILE) tops_of[2] = tops.v[((int64_t)b * p.HK + hk) * nt + min(j0 / TILE + (int)threadIdx.x, nt - 1)];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            tops_of[k] = wave_max(tops_of[k]);
+            if (lane == 0) ls[1][4 * k + wave] = tops_of[k];       // (written again behind the first turn's barrier)
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 3; ++k) tops_of[k] = fmaxf(fmaxf(ls[1][4 * k], ls[1][4 * k + 1]), fmaxf(ls[1][4 * k + 2], ls[1][4 * k + 3]));
+        const int e = __builtin_amdgcn_readfirstlane(shift_of(__builtin_fmaf(tops_of[0], tops_of[2], tops_of[1])));
+        const int room = __builtin_amdgcn_readfirstlane(max(0, 15 - __builtin_amdgcn_frexp_expf(tops_of[2])));
+        of_p = min(max(e, 0), 14);
+        of_v = min(max(e - of_p, -10), room);
+        of_p = min(of_p, e - of_v);
+        const T by = (T)power_of_two(of_v);
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u) v[u] *= by;
+    }
+    const float p_add = of_p * LN2, v_by = power_of_two(of_v);
+    parked += threadIdx.x;
+#pragma unroll
+    for (int x = 0; x < PARKED; ++x) parked[x * NT] = __builtin_bit_cast(u32x4, v[x]);
+    // tile t from tq and tg, its -lse / scale and -rowsum(do o) (with the powers of two) in `stats`, the next one's copies into nq and ng
     const auto turn = [&](int t, const u32x4* tq, const u32x4* tg, float* stats, u32x4* nq, u32x4* ng) __attribute__((always_inline)) {
         const int qn = qt * TILE;
         arrived();
         if (threadIdx.x < TILE) {
             asm volatile("" : "+v"(se), "+v"(sd));
             // (a row past the end, or that sees nothing: every P is 0)
-            stats[threadIdx.x] = si < p.S && se != -INFINITY ? -se * c1 : -INFINITY;
-            stats[TILE + threadIdx.x] = -sd;
+            stats[threadIdx.x] = si < p.S && se != -INFINITY ? (NARROW<T> ? p_add - se : -se) * c1 : -INFINITY;
+            stats[TILE + threadIdx.x] = NARROW<T> ? -sd * v_by : -sd;
         }
         __syncthreads();                       // the tile is there, and the other one is no longer read
         if (t + 1 < t1) {
@@ -601,6 +727,7 @@ DEV void dkv_body(const D8sAttnArgs& p, const float* delta, float* part, KeySpli
         turn(t, lq0, lg0, ls[0], lq1, lg1);
         if (t + 1 < t1) turn(t + 1, lq1, lg1, ls[1], lq0, lg0);
     }
+    const float dk_by = NARROW<T> ? p.scale * power_of_two(-of_p - of_v) : p.scale, dv_by = NARROW<T> ? power_of_two(-of_p) : 1.0f;
     if (!on) {                                 // a masked key's column may hold anything: it has no gradient
 #pragma unroll
         for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
@@ -615,8 +742,8 @@ DEV void dkv_body(const D8sAttnArgs& p, const float* delta, float* part, KeySpli
                 f32x4 x, z;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    x[r] = dk[d][4 * g + r] * p.scale;
-                    z[r] = dv[d][4 * g + r];
+                    x[r] = dk[d][4 * g + r] * dk_by;
+                    z[r] = dv[d][4 * g + r] * dv_by;
                 }
                 *(f32x4*)(o + 32 * d + 8 * g) = x;
                 *(f32x4*)(o + KEYS * D + 32 * d + 8 * g) = z;
@@ -624,21 +751,21 @@ DEV void dkv_body(const D8sAttnArgs& p, const float* delta, float* part, KeySpli
         return;
     }
     const int64_t at = (((int64_t)b * p.S + j) * p.HK + hk) * D;
-    store_rows<T, ND>((T*)p.dk + at, dk, p.scale, j < p.S, lane);
-    store_rows<T, ND>((T*)p.dv + at, dv, 1.0f, j < p.S, lane);
+    store_rows<T, ND>((T*)p.dk + at, dk, dk_by, j < p.S, lane);
+    store_rows<T, ND>((T*)p.dv + at, dv, dv_by, j < p.S, lane);
 }
 
 // The first `of_keys` workgroups run keys, the others queries
 template <class T, int D>
-__global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn_back(D8sAttnArgs p, const float* delta, float* part, KeySplit ks,
-                                                                     int of_keys) {
+__global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn_back(D8sAttnArgs p, const float* delta, Tops tops,
+                                                                     float* part, KeySplit ks, int of_keys) {
     constexpr int N = TILE * D / 8;
     __shared__ u32x4 a0[N], a1[N], b0[N], b1[N];
     __shared__ float stats[2][2 * TILE];
     __shared__ u32x4 parked[PARKED * NT];
     const int w = blockIdx.x;
-    if (w < of_keys) dkv_body<T, D>(p, delta, part, ks, xcd_order(w, of_keys), a0, a1, b0, b1, stats, parked);
-    else dq_body<T, D>(p, delta, xcd_order(w - of_keys, gridDim.x - of_keys), a0, a1, b0, b1);
+    if (w < of_keys) dkv_body<T, D>(p, delta, tops, part, ks, xcd_order(w, of_keys), a0, a1, b0, b1, stats, parked);
+    else dq_body<T, D>(p, delta, tops, xcd_order(w - of_keys, gridDim.x - of_keys), a0, a1, b0, b1);
 }
 
 // dk and dv of the split tiles: the float32 parts summed in order, four values a thread
@@ -683,6 +810,11 @@ int64_t key_items(const D8sAttnArgs* a, const KeySplit& k) {
     return (int64_t)k.sink_tiles * k.sink_split + (nk - k.sink_tiles) * k.split;
 }
 uint64_t delta_bytes(const D8sAttnArgs* a) { return ((uint64_t)a->B * a->H * a->S * 4 + 255) / 256 * 256; }
+// The tiles' largest norms, where dS is brought into its type's range
+uint64_t tops_bytes(const D8sAttnArgs* a) {
+    if (a->dtype != D8S_F16) return 0;
+    return ((uint64_t)a->B * (2 * a->H + a->HK) * ((a->S + TILE - 1) / TILE) * 4 + 255) / 256 * 256;
+}
 
 // ---- one new token against a cache ------------------------------------------------------------------
 // A workgroup runs GM query heads of a key head over a share of the keys their token sees.  A key's row is read 16
@@ -886,14 +1018,18 @@ void attn_run(const D8sAttnArgs& a, hipStream_t st) {
 template <class T, int D>
 void attn_back_run(const D8sAttnArgs& a, hipStream_t st) {
     float* delta = (float*)a.workspace;
-    float* part = (float*)((char*)a.workspace + delta_bytes(&a));
+    float* top = (float*)((char*)a.workspace + delta_bytes(&a));
+    float* part = (float*)((char*)top + tops_bytes(&a));
+    const int64_t tiles = (a.S + TILE - 1) / TILE;
+    const Tops tops = {top, top + a.B * a.H * tiles, top + 2 * a.B * a.H * tiles};
     const KeySplit ks = key_split(&a);
     const int problems = a.B * a.HK, nk = (a.S + KEYS - 1) / KEYS;
     const int joined = ks.split > 1 ? nk : ks.sink_split > 1 ? ks.sink_tiles : 0;
     const int of_keys = problems * (int)key_items(&a, ks), of_queries = a.B * a.H * ((a.S + 127) / 128);
-    constexpr int ROWS = NT / (D / 8);
-    hipLaunchKernelGGL((k_attn_delta<T, D>), dim3((unsigned)(a.B * a.H * ((a.S + ROWS - 1) / ROWS))), dim3(NT), 0, st, a, delta);
-    hipLaunchKernelGGL((k_attn_back<T, D>), dim3((unsigned)(of_keys + of_queries)), dim3(NT), 0, st, a, delta, part, ks, of_keys);
+    constexpr int ROWS = NARROW<T> ? TILE : NT / (D / 8);
+    const unsigned deltas = (unsigned)(a.B * (a.H + (NARROW<T> ? a.HK : 0)) * ((a.S + ROWS - 1) / ROWS));
+    hipLaunchKernelGGL((k_attn_delta<T, D>), dim3(deltas), dim3(NT), 0, st, a, delta, tops);
+    hipLaunchKernelGGL((k_attn_back<T, D>), dim3((unsigned)(of_keys + of_queries)), dim3(NT), 0, st, a, delta, tops, part, ks, of_keys);
     if (joined)
         hipLaunchKernelGGL((k_attn_join<T, D>), dim3((unsigned)(problems * joined), 2 * KEYS * D / (4 * NT)), dim3(NT), 0, st,
                            a, part, ks);
@@ -933,7 +1069,7 @@ extern "C" int d8s_attention_workspace(const D8sAttnArgs* a, uint64_t* bytes) {
     AREQ(bytes != nullptr, "null arguments");
     const KeySplit k = key_split(a);
     const bool parts = k.split > 1 || (k.sink_tiles > 0 && k.sink_split > 1);
-    *bytes = delta_bytes(a) + (parts ? (uint64_t)a->B * a->HK * key_items(a, k) * 2 * KEYS * a->D * 4 : 0);
+    *bytes = delta_bytes(a) + tops_bytes(a) + (parts ? (uint64_t)a->B * a->HK * key_items(a, k) * 2 * KEYS * a->D * 4 : 0);
     return 0;
 }
 

@@ -1,0 +1,117 @@
+"""Attention's gradients in float16 over the range of gradients that training gives: a loss averaged over thousands of
+tokens, a loss scaled up, a few rows far larger than the others.
+
+The oracle is the formula in float64, and errors are compared by their norm.  With u = 2^-11 (a float16 rounding is off
+by at most u of the value, its own last step 2^-25 below 2^-14), every rounded value is off by its own independent
+error, so the norm of a sum of n of them is at most u times the root of the sum of the terms' squares (their root mean
+square is below 0.6 u).  What is rounded: dS (or P, for dv) before the product, out before rowsum(do out), the result;
+P has an error of es beside, from its score in float32."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from rsna_knee_efficiency_amd import context
+
+pytestmark = pytest.mark.gpu
+
+U, STEP = 2.0 ** -11, 2.0 ** -25
+
+
+def _heads(t, per=1):
+    return t.double().transpose(1, 2).repeat_interleave(per, 1)
+
+
+def _oracle(q, k, v, dout, see, scale):
+    """(dq, dk, dv) in float64 as (batch, heads, tokens, channels) and the norms their errors stay below"""
+    b, n, h, d = q.shape
+    per = h // k.shape[2]
+    q, k, v, do = _heads(q), _heads(k, per), _heads(v, per), _heads(dout)
+    s = (q @ k.transpose(2, 3) * scale).masked_fill(~see, -math.inf)
+    es = 2 * d * 2.0 ** -24 * (q.norm(dim=-1).amax() * k.norm(dim=-1).amax()) * scale + 2.0 ** -19
+    p = torch.where(see, torch.softmax(s, -1), 0.0)          # (a row that sees nothing: zeros)
+    o = p @ v
+    row = (do * o).sum(-1, keepdim=True)
+    ds = p * (do @ v.transpose(2, 3) - row)
+    u = U + 2 * es
+    # out's own rounding, and that of the P it came from
+    erow = ((do * o).square().sum(-1, keepdim=True) + (do.square() * (p.square() @ v.square())).sum(-1, keepdim=True)).sqrt() * u
+
+    def shared(t):
+        return t.reshape(b, -1, per, *t.shape[2:]).sum(2)
+    dq, dk, dv = ds @ k * scale, shared(ds.transpose(2, 3) @ q) * scale, shared(p.transpose(2, 3) @ do)
+
+    def bound(want, left, right, by):
+        terms = (left.square() @ right.square()).sum().sqrt() * by
+        return U * want.norm() + STEP * math.sqrt(want.numel()) + u * terms
+    edq = bound(dq, ds, k, scale) + ((p @ k) * erow).norm() * scale
+    edk = bound(dk, ds.transpose(2, 3), q, scale) + ((p.transpose(2, 3) @ (erow * q)).norm()) * scale
+    edv = bound(dv, p.transpose(2, 3), do, 1.0)
+    return (dq, dk, dv), (edq, edk, edv)
+
+
+def _check(q, k, v, dout, scale=None, mask=None, **how):
+    n = q.shape[1]
+    how = dict(left=None, right=None, sinks=0) | how
+    i, j = torch.arange(n, device=q.device)[:, None], torch.arange(n, device=q.device)[None]
+    left, right = (n if how[side] is None else how[side] for side in ("left", "right"))
+    see = (j <= i + right) & ((j >= i - left) | (j < how["sinks"]))
+    see = see[None, None] if mask is None else see[None, None] & mask[:, None, None]
+    out, lse = context.window_attention_forward(q, k, v, **how, key_mask=mask, scale=scale)
+    got = context.window_attention_backward(dout, q, k, v, out, lse, **how, key_mask=mask, scale=scale)
+    want, tol = _oracle(q, k, v, dout, see, 1 / math.sqrt(q.shape[-1]) if scale is None else scale)
+    for name, x, y, e in zip(("dq", "dk", "dv"), got, want, tol):
+        off = (x.double().transpose(1, 2) - y).norm()
+        print(f"{name}: off by {(off / y.norm()).item():.2e}, bound {(e / y.norm()).item():.2e} of its norm", flush=True)
+        assert off <= e, name
+    return got
+
+
+def _inputs(dev, seed, b, n, h, hk, d, size, qs=1.5, vs=1.0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    shapes = ((b, n, h, d), (b, n, hk, d), (b, n, hk, d), (b, n, h, d))
+    return [(torch.randn(s, generator=g, device=dev) * x).half() for s, x in zip(shapes, (qs, 1.0, vs, size))]
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-3, 1e-4, 1e-5])
+@pytest.mark.parametrize("d,h,hk", [(64, 1, 1), (128, 2, 1)])
+def test_gradients_of_an_averaged_loss(dev, size, d, h, hk):
+    """Thousands of visible keys: dS is a thousandth of a gradient that is small by itself."""
+    _check(*_inputs(dev, 1, 1, 3000, h, hk, d, size))
+    _check(*_inputs(dev, 2, 1, 3001, h, hk, d, size), left=1000, right=0, sinks=5)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_gradients_of_a_scaled_loss(dev, d):
+    """dP beyond float16's largest value, results within it."""
+    q, k, v, do = _inputs(dev, 3, 2, 16, 2, 1, d, 1e4, qs=4.0, vs=8.0)
+    got = _check(q, k, v, do, scale=2.0 ** -7)
+    assert all(t.isfinite().all() for t in got)
+
+
+def test_rows_of_all_sizes(dev):
+    """Summary tokens whose gradient is ten thousand times the others', and rows whose gradient is zero."""
+    q, k, v, do = _inputs(dev, 4, 1, 2000, 2, 2, 64, 1e-4)
+    do[:, :4] *= 1e4
+    do[:, 500:700] = 0
+    _check(q, k, v, do, left=600, right=600, sinks=4)
+    _check(q, k, v, torch.zeros_like(do), left=600, right=600, sinks=4)
+
+
+def test_unseen_rows_cost_nothing(dev):
+    """What a masked key holds, and the gradient of a query that sees nothing, cost the others no bits."""
+    q, k, v, do = _inputs(dev, 5, 1, 700, 2, 1, 64, 1e-4)
+    mask = torch.ones((1, 700), dtype=torch.bool, device=dev)
+    mask[:, 100:300] = False
+    how = dict(left=20, right=20, sinks=0)
+    want = _check(q, k, v, do, mask=mask, **how)
+    far_do = do.clone()
+    far_do[:, 120:280] = 6e4                   # these see masked keys only
+    for x in (6e4, float("inf"), float("nan")):
+        far_v = v.clone()
+        far_v[:, 100:300] = x
+        out, lse = context.window_attention_forward(q, k, far_v, **how, key_mask=mask)
+        got = context.window_attention_backward(far_do, q, k, far_v, out, lse, **how, key_mask=mask)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), x
