@@ -186,6 +186,15 @@ struct Copy {
             if (!(rows >> (row + n * STEP) & 1)) tile[n * NT + threadIdx.x] = u32x4{0, 0, 0, 0};
     }
 };
+// The same for a loop that seldom needs it: nothing of it is held in registers from turn to turn
+template <int D>
+DEV void clear_rows(u32x4* a, u32x4* b, uint64_t rows) {
+    int at = threadIdx.x;
+    asm volatile("" : "+v"(at));
+#pragma unroll 1
+    for (; at < TILE * D / 8; at += NT)
+        if (!(rows >> (at / (D / 8)) & 1)) a[at] = b[at] = u32x4{0, 0, 0, 0};
+}
 DEV void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // Which of the tile's keys exist and are not masked, from the byte a lane read for its key
@@ -391,6 +400,8 @@ DEV float wave_max(float x) {
 DEV int shift_of(float bound) {
     return bound > 0.0f && bound < INFINITY ? min(max(14 - __builtin_amdgcn_frexp_expf(bound), -64), 64) : 0;
 }
+// A value that is the same in all lanes, in a scalar register
+DEV float uniform(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
 DEV float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 // The sum of squares of a row whose other half is held by the lane 32 away
 template <class T, int N>
@@ -570,9 +581,10 @@ struct KeySplit {
 };
 constexpr int KEYS = 128;
 // Operands of v that lie in LDS, each lane's own, and are read again for every product: with all of k, v, dk and dv in
-// registers nine of a lane's are spilled at D = 128, and a read back from scratch memory waits for the copies in
-// flight before it.
-constexpr int PARKED = 3;
+// registers nine of a lane's are spilled at D = 128 (four at D = 64 in float16, whose powers of two take some), and a
+// read back from scratch memory waits for the copies in flight before it.
+template <class T, int D>
+constexpr int PARKED = NARROW<T> && D == 64 ? 4 : 3;
 
 template <class T, int D>
 DEV void dkv_body(const D8sAttnArgs& p, const float* delta, const Tops& tops, float* part, KeySplit ks, int id, u32x4* lq0, u32x4* lq1, u32x4* lg0,
@@ -613,13 +625,11 @@ DEV void dkv_body(const D8sAttnArgs& p, const float* delta, const Tops& tops, fl
     const auto load = [&](u32x4* nq, u32x4* ng) __attribute__((always_inline)) {
         copy((const uint16_t*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, qt * TILE, p.S - 1, nq, wave);
         copy((const uint16_t*)p.dout + b * p.do_sb + h * p.do_sh, p.do_ss, qt * TILE, p.S - 1, ng, wave);
-        if (threadIdx.x < TILE) {
-            const int i = qt * TILE + threadIdx.x;
-            const int64_t at = ((int64_t)b * p.H + h) * p.S + min(i, p.S - 1);
-            se = p.lse[at];
-            sd = delta[at];
-            si = i;
-        }
+        const int i = qt * TILE + lane;
+        const int64_t at = ((int64_t)b * p.H + h) * p.S + min(i, p.S - 1);
+        se = p.lse[at];
+        if (wave == 0) sd = delta[at];
+        si = i;
     };
     if (t0 < t1) load(lq0, lg0);
     // The powers of two (exponents) of P and of v, which dS then has both of: P's between 0 and 14 as far as v can take the
@@ -652,19 +662,24 @@ DEV void dkv_body(const D8sAttnArgs& p, const float* delta, const Tops& tops, fl
 #pragma unroll
         for (int u = 0; u < D / 16; ++u) v[u] *= by;
     }
-    const float p_add = of_p * LN2, v_by = power_of_two(of_v);
+    const float p_add = uniform(of_p * LN2), v_by = power_of_two(of_v);
     parked += threadIdx.x;
 #pragma unroll
-    for (int x = 0; x < PARKED; ++x) parked[x * NT] = __builtin_bit_cast(u32x4, v[x]);
+    for (int x = 0; x < PARKED<T, D>; ++x) parked[x * NT] = __builtin_bit_cast(u32x4, v[x]);
     // tile t from tq and tg, its -lse / scale and -rowsum(do o) (with the powers of two) in `stats`, the next one's copies into nq and ng
-    const auto turn = [&](int t, const u32x4* tq, const u32x4* tg, float* stats, u32x4* nq, u32x4* ng) __attribute__((always_inline)) {
+    const auto turn = [&](int t, u32x4* tq, u32x4* tg, float* stats, u32x4* nq, u32x4* ng) __attribute__((always_inline)) {
         const int qn = qt * TILE;
         arrived();
-        if (threadIdx.x < TILE) {
-            asm volatile("" : "+v"(se), "+v"(sd));
-            // (a row past the end, or that sees nothing: every P is 0)
-            stats[threadIdx.x] = si < p.S && se != -INFINITY ? (NARROW<T> ? p_add - se : -se) * c1 : -INFINITY;
-            stats[TILE + threadIdx.x] = NARROW<T> ? -sd * v_by : -sd;
+        asm volatile("" : "+v"(se), "+v"(sd));
+        // a row past the end, or that sees nothing: every P is 0, and whatever memory holds of it is not used
+        const bool sees = si < p.S && se != -INFINITY;
+        if (mask) {                            // (without one, a query sees itself)
+            const uint64_t rows = __ballot(sees);
+            if (rows != ~0ull) clear_rows<D>(tq, tg, rows);
+        }
+        if (wave == 0) {
+            stats[lane] = sees ? (NARROW<T> ? p_add - se : -se) * c1 : -INFINITY;
+            stats[TILE + lane] = sees ? (NARROW<T> ? -sd * v_by : -sd) : 0.0f;
         }
         __syncthreads();                       // the tile is there, and the other one is no longer read
         if (t + 1 < t1) {
@@ -694,7 +709,7 @@ DEV void dkv_body(const D8sAttnArgs& p, const float* delta, const Tops& tops, fl
 #pragma unroll
             for (int x = 0; x < D / 16; ++x) {
                 s = mfma(rows_frag<T, D>(tq, ra, 32 * u, x), k[x], s);
-                dp = mfma(rows_frag<T, D>(tg, ra, 32 * u, x), x < PARKED ? __builtin_bit_cast(Frag<T>, parked[fresh(x * NT)]) : v[x], dp);
+                dp = mfma(rows_frag<T, D>(tg, ra, 32 * u, x), x < PARKED<T, D> ? __builtin_bit_cast(Frag<T>, parked[fresh(x * NT)]) : v[x], dp);
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -762,7 +777,7 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn_back(D8sAttnArgs
     constexpr int N = TILE * D / 8;
     __shared__ u32x4 a0[N], a1[N], b0[N], b1[N];
     __shared__ float stats[2][2 * TILE];
-    __shared__ u32x4 parked[PARKED * NT];
+    __shared__ u32x4 parked[PARKED<T, D> * NT];
     const int w = blockIdx.x;
     if (w < of_keys) dkv_body<T, D>(p, delta, tops, part, ks, xcd_order(w, of_keys), a0, a1, b0, b1, stats, parked);
     else dq_body<T, D>(p, delta, tops, xcd_order(w - of_keys, gridDim.x - of_keys), a0, a1, b0, b1);

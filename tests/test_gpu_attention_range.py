@@ -115,3 +115,28 @@ def test_unseen_rows_cost_nothing(dev):
         out, lse = context.window_attention_forward(q, k, far_v, **how, key_mask=mask)
         got = context.window_attention_backward(far_do, q, k, far_v, out, lse, **how, key_mask=mask)
         assert all(torch.equal(a, b) for a, b in zip(got, want)), x
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.float16, 64), (torch.float16, 128), (torch.bfloat16, 64), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_unseen_rows_are_not_used(dev, dtype, d, bad):
+    """Queries that see nothing, and their gradient, may hold anything: no other row's gradient changes, theirs are zeros."""
+    q, k, v, do = (t.to(dtype) for t in _inputs(dev, 6, 2, 500, 4, 2, d, 1.0))
+    mask = torch.ones((2, 500), dtype=torch.bool, device=dev)
+    mask[:, 100:300] = False
+    mask[1, 310:] = False
+    for left, right, sinks in ((20, 20, 0), (5, 0, 0)):
+        how = dict(left=left, right=right, sinks=sinks, key_mask=mask)
+        out, lse = context.window_attention_forward(q, k, v, **how)
+        want = context.window_attention_backward(do, q, k, v, out, lse, **how)
+        assert all(t.isfinite().all() for t in want)
+        unseen = (lse == -math.inf)[:, 0]
+        assert unseen[:, 130:270].all() and unseen[1, 340:].all()
+        for both in ((True, False), (False, True), (True, True)):
+            far = [t.clone() for t in (q, do)]
+            for t, on in zip(far, both):
+                t[unseen] = bad if on else t[unseen]
+            again = context.window_attention_forward(far[0], k, v, **how)
+            assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+            got = context.window_attention_backward(far[1], far[0], k, v, out, lse, **how)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)) and not got[0][unseen].any()
