@@ -91,9 +91,11 @@ class AdamW:
             which = [i for i, g in enumerate(grads) if g is not None]
             params, grads, shapes, dtypes = ([x[i] for i in which] for x in (params, grads, shapes, dtypes))
             table = table[which]
-        if [p.shape for p in params] != shapes or [p.dtype for p in params] != dtypes or not all(p.is_contiguous() for p in params):
-            raise ValueError("a parameter has changed")
-        if [g.shape for g in grads] != shapes or any(g.device != self.device for g in grads):
+        on = self.device.index                 # (the kernel follows raw pointers: a moved parameter's is another device's)
+        if ([p.shape for p in params] != shapes or [p.dtype for p in params] != dtypes
+                or not all(p.get_device() == on and p.is_contiguous() for p in params)):
+            raise ValueError("a parameter has changed its shape, type, layout or device")
+        if [g.shape for g in grads] != shapes or any(g.get_device() != on for g in grads):
             raise ValueError("a gradient must have its parameter's shape and device")
         kinds = list(zip(dtypes, [g.dtype for g in grads]))
         for pt, gt in set(kinds):
