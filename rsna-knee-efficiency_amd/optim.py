@@ -5,7 +5,8 @@ context layer, with moments in 32 or 8 bits.
     loss.backward()
     opt.step()                           # or opt.step(grads), opt.step(grad_scale=scale on the GPU)
 
-A step is one launch for every 100 tensors of one pair of types, whatever their sizes.  There is no CPU path: without
+A step is one launch for every 100 tensors of one pair of types (and, where some were left out of earlier steps, of one
+step number), whatever their sizes.  There is no CPU path: without
 the library the calls raise.
 """
 from __future__ import annotations
@@ -21,7 +22,8 @@ _ROW = np.dtype([("p", "u8"), ("g", "u8"), ("n", "i8"), ("at", "i8")])       # A
 class AdamW:
     """p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps) after
     m = beta1 m + (1 - beta1) g and v = beta2 v + (1 - beta2) g^2, all in float32 with every operation rounded by
-    itself, p then to its type.
+    itself, p then to its type.  t counts a tensor's own steps (`steps`): one that is left out of a step keeps its
+    number with its moments.
 
     params: contiguous float32, bfloat16 or float16 tensors on one GPU; gradients are float32 or 16 bits beside
     float32 parameters, float32 or the parameter's own type beside 16-bit ones.  The moments of all tensors lie in
@@ -45,7 +47,9 @@ class AdamW:
         for p in self.params:
             self._check(p)
         self.lr, self.betas, self.eps, self.weight_decay, self.state_bits = lr, tuple(betas), eps, weight_decay, state_bits
-        self.step_count = 0
+        self.step_count = 0                    # calls of `step`
+        # the number of steps of every tensor: one for all as long as none is left out of one, else a list
+        self._steps: int | list[int] = 0
         block = hip.ADAMW_BLOCK
         self._table = np.zeros(len(self.params), _ROW)
         self._table["n"] = [p.numel() for p in self.params]
@@ -67,9 +71,14 @@ class AdamW:
         if p.dtype not in hip.ELEMENTS or not p.is_contiguous() or p.device != self.device or p.device.type != "cuda":
             raise ValueError("parameters must be contiguous float32, bfloat16 or float16 tensors on one GPU")
 
+    @property
+    def steps(self) -> list[int]:
+        """How many steps each tensor has taken."""
+        return [self._steps] * len(self.params) if isinstance(self._steps, int) else list(self._steps)
+
     def step(self, grads=None, grad_scale: torch.Tensor | None = None) -> None:
         """One step in place.  grads: a tensor, or None, for every parameter (default: their .grad); parameters
-        without one are left as they are, their moments too.  grad_scale: one float32 on the GPU that every
+        without one are left as they are, their moments and their number of steps too.  grad_scale: one float32 on the GPU that every
         gradient is multiplied by.  The step's numbers are arguments of its launches, so it cannot be recorded into
         a graph."""
         grads = [p.grad for p in self.params] if grads is None else list(grads)
@@ -105,13 +114,25 @@ class AdamW:
         table["p"], table["g"] = [p.data_ptr() for p in params], [g.data_ptr() for g in grads]
         s = self._state
         at = [t.data_ptr() for t in s.values()] + [0] * (4 - len(s))
-        for kind in dict.fromkeys(kinds):
-            rows = table if kinds.count(kind) == len(kinds) else table[[i for i, x in enumerate(kinds) if x == kind]]
+        if which is None and isinstance(self._steps, int):
+            numbers, after = [self._steps + 1], self._steps + 1
+            groups = kinds
+        else:
+            after = self.steps
+            for i in range(len(after)) if which is None else which:
+                after[i] += 1
+            numbers = after if which is None else [after[i] for i in which]
+            groups = list(zip(kinds, numbers))
+            after = after[0] if len(set(after)) == 1 else after
+        for group in dict.fromkeys(groups):
+            rows = table if groups.count(group) == len(groups) else table[[i for i, x in enumerate(groups) if x == group]]
+            (pt, gt), number = (group, numbers[0]) if groups is kinds else group
             hip.launch("d8s_adamw", self.device, hip.AdamwArgs(
-                rows.ctypes.data, *at, 0 if grad_scale is None else grad_scale.data_ptr(), self.step_count + 1, self.lr,
-                *self.betas, self.eps, self.weight_decay, len(rows), hip.ELEMENTS[kind[0]], hip.ELEMENTS[kind[1]],
+                rows.ctypes.data, *at, 0 if grad_scale is None else grad_scale.data_ptr(), number, self.lr,
+                *self.betas, self.eps, self.weight_decay, len(rows), hip.ELEMENTS[pt], hip.ELEMENTS[gt],
                 self.state_bits))
         self.step_count += 1
+        self._steps = after
         torch.autograd.graph.increment_version([*params, *s.values()])
 
     def moments(self) -> tuple[torch.Tensor, torch.Tensor]:
@@ -130,18 +151,23 @@ class AdamW:
             p.grad = None
 
     def state_dict(self) -> dict:
-        """The step count and copies of the moments as they are kept."""
-        return {"step": self.step_count, **{n: t.clone() for n, t in self._state.items()}}
+        """The step counts, of calls and of every tensor, and copies of the moments as they are kept."""
+        return {"step": self.step_count, "steps": self.steps, **{n: t.clone() for n, t in self._state.items()}}
 
     def load_state_dict(self, state: dict) -> None:
-        """Takes over what `state_dict` gave of an optimizer over tensors of the same sizes and state_bits."""
-        if set(state) != {"step", *self._state}:
-            raise ValueError(f"the state must hold step and {sorted(self._state)}")
+        """Takes over what `state_dict` gave of an optimizer over tensors of the same sizes and state_bits.  Without
+        "steps" every tensor has taken "step" of them."""
+        if set(state) - {"steps"} != {"step", *self._state}:
+            raise ValueError(f"the state must hold step, steps and {sorted(self._state)}")
         for n, t in self._state.items():
             if state[n].shape != t.shape or state[n].dtype != t.dtype:
                 raise ValueError(f"{n} must be {tuple(t.shape)} {t.dtype}")
-        if int(state["step"]) < 0:
+        step = int(state["step"])
+        steps = [int(t) for t in state["steps"]] if "steps" in state else [step] * len(self.params)
+        if step < 0 or any(t < 0 for t in steps):
             raise ValueError("step must not be negative")
+        if len(steps) != len(self.params):
+            raise ValueError("steps must hold a number for every parameter")
         for n, t in self._state.items():
             t.copy_(state[n])
-        self.step_count = int(state["step"])
+        self.step_count, self._steps = step, steps[0] if len(set(steps)) == 1 else steps
