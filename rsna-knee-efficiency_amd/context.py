@@ -6,7 +6,8 @@ The reference's head attends over one feature vector a window, at most 128 of th
 row and column; its attention is kept to a window of neighbours and a few first summary tokens.  Each operator has a
 differentiable form (`layer_norm`, `rotary`, `window_attention`), the forward and backward calls it is made of, and
 for tokens that arrive one at a time `window_attention_token`.  Calls run on the current stream and may be recorded
-into HIP graphs.  There is no CPU path: without the library the calls raise.
+into HIP graphs.  There is no CPU path: without the library the calls raise.  Tensors with a forward-mode tangent are
+refused.
 """
 from __future__ import annotations
 
@@ -14,6 +15,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import hip
 
@@ -28,6 +30,15 @@ def _on_gpu(first: torch.Tensor, *others: torch.Tensor) -> None:
     for t in others:
         if t.get_device() != index:
             _fail("the tensors must be on one GPU")
+
+
+def _no_tangents(*tensors: torch.Tensor | None) -> None:
+    """Every call begins with this: a kernel would leave out a forward-mode tangent without a word (a tensor that has one
+    need not require a gradient)."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("forward-mode derivatives are not implemented: a tensor has a tangent")
 
 
 def _like(x: torch.Tensor) -> torch.Tensor:
@@ -63,6 +74,7 @@ def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor
     """x (..., width) in float32, bfloat16 or float16; weight and bias (width,) in float32 or x's type ->
     (y like x, mean, rstd), the last two float32, one a row, for `layer_norm_backward` (None without
     `statistics`)."""
+    _no_tangents(x, weight, bias)
     width, dtype, wdtype = _norm_types(x, weight)
     if bias is not None and (bias.shape != weight.shape or bias.dtype != weight.dtype):
         _fail("bias must be like weight")
@@ -87,6 +99,7 @@ def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, mean: torch.Tensor,
                         rstd: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The gradients (dx like x, dweight, dbias like weight) of `layer_norm_forward` at dy like x."""
+    _no_tangents(dy, x, weight, mean, rstd)
     width, dtype, wdtype = _norm_types(x, weight)
     n = x.numel() // width
     if dy.shape != x.shape or dy.dtype != x.dtype:
@@ -128,6 +141,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     """Layer norm over x's last dimension, differentiable in x, weight and bias (types as in
     `layer_norm_forward`)."""
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        _no_tangents(x, weight, bias)
         return _LayerNorm.apply(x, weight, bias, eps)
     return layer_norm_forward(x, weight, bias, eps, statistics=False)[0]
 
@@ -154,6 +168,7 @@ def _rotary_plan(sections: tuple, base: float) -> bytes:
 
 
 def _rotate(x, positions, sections, base, adjacent, inverse, out):
+    _no_tangents(x, positions, out)
     a = hip.RotaryArgs.from_buffer_copy(_rotary_plan(tuple(sections), float(base)))
     if x.dim() != 4 or x.dtype not in hip.ELEMENTS or x.shape[3] < 2 * a.pairs:
         _fail(f"x must be (batch, tokens, heads, channels) of at least {2 * a.pairs} channels in float32, bfloat16 or "
@@ -205,6 +220,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, sections, base: float = 100
     call is differentiable in x).  `out` may be x itself, where no gradient is asked for.  Queries and keys that lie
     beside each other in one tensor are turned in one call, as x of all their heads."""
     if torch.is_grad_enabled() and x.requires_grad:
+        _no_tangents(x, positions, out)
         if out is not None:
             _fail("out is not taken where x requires a gradient")
         return _Rotary.apply(x, positions, tuple(sections), base, adjacent, inverse)
@@ -274,6 +290,7 @@ def window_attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
 
     -> (out like q, lse (batch, heads, tokens) float32: the logarithm of the sum of exponentials, -inf where nothing
     is seen; None without `statistics`)"""
+    _no_tangents(q, k, v)
     a, _kept = _attn_args(q, k, v, left, right, sinks, key_mask, scale)
     out = _like(q)
     lse = q.new_empty((a.B, a.H, a.S), dtype=torch.float32) if statistics else None
@@ -287,6 +304,7 @@ def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
                               lse: torch.Tensor, left: int | None = None, right: int | None = 0, sinks: int = 0,
                               key_mask: torch.Tensor | None = None, scale: float | None = None) -> tuple:
     """The gradients (dq, dk, dv) of `window_attention_forward` at dout like out."""
+    _no_tangents(dout, q, k, v, out, lse)
     a, _kept = _attn_args(q, k, v, left, right, sinks, key_mask, scale)
     if dout.shape != q.shape or dout.dtype != q.dtype or out.shape != q.shape or out.dtype != q.dtype:
         _fail("dout and out must be like q")
@@ -326,6 +344,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: in
                      sinks: int = 0, key_mask: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
     """`window_attention_forward`'s out, differentiable in q, k and v."""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        _no_tangents(q, k, v)
         return _WindowAttention.apply(q, k, v, left, right, sinks, key_mask, scale)
     return window_attention_forward(q, k, v, left, right, sinks, key_mask, scale, statistics=False)[0]
 
@@ -337,6 +356,7 @@ def window_attention_token(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     the GPU) tokens in its cache, whose keys and values are already there; it sees the last left + 1 of them and the
     first `sinks`.  Lengths are not checked (that would synchronise): they are taken as 0 .. capacity, and length 0
     gives zeros.  What the cache holds from a row's length on is not read."""
+    _no_tangents(q, k_cache, v_cache)
     if q.dim() != 3 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
         _fail("q must be (batch, heads, channels), k_cache and v_cache (batch, capacity, key heads, channels)")
     B, H, D = q.shape
