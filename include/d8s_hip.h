@@ -512,7 +512,8 @@ int d8s_rotary(const D8sRotaryArgs* a, void* stream);
 
 /* Attention of S tokens within a window and `sinks` first tokens: key j is visible to query i iff j <= i + right,
  * (j >= i - left or j < sinks) and mask[j] is not 0 (mask 0: all).  A query that sees nothing has zeros, lse -inf
- * and no gradient; what lies in rows of masked keys is not used.  q, dout [B][S][H][D], k, v [B][S][HK][D] of dtype
+ * and no gradient (zeros and -inf also where every score it sees is -infinity); what lies in rows of masked keys is
+ * not used.  q, dout [B][S][H][D], k, v [B][S][HK][D] of dtype
  * (D8S_BF16 or D8S_F16; D 64 or 128; H a multiple of HK, query head h uses key head h / (H / HK)) with the given
  * strides (elements, the last dimension contiguous); out, dq [B][S][H][D], dk, dv [B][S][HK][D] and lse [B][H][S]
  * (natural logarithm of the sum of exponentials) contiguous.  Products are of 16 bits with float32 sums; P and dS
@@ -541,7 +542,8 @@ int d8s_attention_backward(const D8sAttnArgs* a, void* stream);
 
 /* One new token a row against a cache: q [B][H][D], k, v [B][S][HK][D] with strides as above; the token is the last
  * of its row's lengths[b] (0 .. S, on the device; others are cut to that) and sees keys as in d8s_attention with
- * right 0 and no mask.  Keys from lengths[b] on are not read.  out [B][H][D] contiguous; length 0 gives zeros.
+ * right 0 and no mask.  Keys from lengths[b] on are not read.  out [B][H][D] contiguous; length 0, or scores of -infinity
+ * alone, give zeros.
  * `workspace`: device memory of d8s_attention_token_workspace bytes (may be 0). */
 typedef struct D8sTokenArgs {
     const void *q, *k, *v;

@@ -355,7 +355,7 @@ def window_attention_token(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     heads, channels), types as in `window_attention_forward`.  Row b's token is the last of the lengths[b] (int32, on
     the GPU) tokens in its cache, whose keys and values are already there; it sees the last left + 1 of them and the
     first `sinks`.  Lengths are not checked (that would synchronise): they are taken as 0 .. capacity, and length 0
-    gives zeros.  What the cache holds from a row's length on is not read."""
+    (or scores that are all -infinity) gives zeros.  What the cache holds from a row's length on is not read."""
     _no_tangents(q, k_cache, v_cache)
     if q.dim() != 3 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
         _fail("q must be (batch, heads, channels), k_cache and v_cache (batch, capacity, key heads, channels)")

@@ -236,6 +236,10 @@ DEV void store_rows(T* o, const f32x16* acc, float scale, bool on, int lane) {
         }
 }
 
+// Whether anything is seen, by the sum of the weights: not where it is zero (no key, or every score is -infinity); a sum that
+// is not a number stays one
+DEV bool any_weight(float sum) { return sum > 0.0f || sum != sum; }
+
 // ---- forward --------------------------------------------------------------------------------------
 // Bound by its instructions: a wave's tile of 32 x 64 scores is 162 vector operations (32 exponentials among them) beside 16
 // (D = 64) or 32 (D = 128) products of 32 cycles, and the two overlap only between waves.  Measured: 22528 tokens of 4
@@ -360,7 +364,7 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
     float l0, l1;
     swap32(l, l0, l1);
     l = l0 + l1;
-    const bool any = l > 0.0f || l != l;       // (a sum that is not a number stays one)
+    const bool any = any_weight(l);
     if (p.lse && lane < 32 && i < p.S) p.lse[((int64_t)b * p.H + h) * p.S + i] = any ? (m * c + log2f(l)) * LN2 : -INFINITY;
     store_rows<T, ND>((T*)p.out + (((int64_t)b * p.S + i) * p.H + h) * D, acc, any ? 1.0f / l : 0.0f, i < p.S, lane);
 }
@@ -945,7 +949,7 @@ __global__ __launch_bounds__(NT) void k_token(D8sTokenArgs p, int split, float* 
         }
         const int64_t head = (int64_t)b * p.H + hk * G + g0 + g;
         if (split == 1) {
-            ((T*)p.out)[head * D + d] = (T)(len > 0 ? o / sum : 0.0f);
+            ((T*)p.out)[head * D + d] = (T)(any_weight(sum) ? o / sum : 0.0f);
         } else {                               // part[share][head][m, l, o ...]
             float* t = part + ((int64_t)cut * p.B * p.H + head) * (D + 2);
             if (d == 0) {
@@ -986,7 +990,7 @@ __global__ __launch_bounds__(NT) void k_join(const float* part, T* out, int spli
         o += so[x][d];
         sum += ss[x];
     }
-    out[(int64_t)head * D + d] = (T)(sum > 0.0f || sum != sum ? o / sum : 0.0f);
+    out[(int64_t)head * D + d] = (T)(any_weight(sum) ? o / sum : 0.0f);
 }
 
 // Shares of a token's keys: enough workgroups for TOKEN_WGS a compute unit, so that long and short rows even out (the 64
