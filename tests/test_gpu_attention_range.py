@@ -140,3 +140,10 @@ def test_unseen_rows_are_not_used(dev, dtype, d, bad):
             assert torch.equal(again[0], out) and torch.equal(again[1], lse)
             got = context.window_attention_backward(far[1], far[0], k, v, out, lse, **how)
             assert all(torch.equal(a, b) for a, b in zip(got, want)) and not got[0][unseen].any()
+
+
+def test_many_first_tokens(dev):
+    """More tiles of first tokens than the GPU needs workgroups: their gradients are split into few shares."""
+    q, k, v, do = _inputs(dev, 7, 1, 4000, 16, 8, 64, 1e-3)
+    _check(q, k, v, do, left=3, right=0, sinks=4000)
+    _check(q, k, v, do, left=100, right=0, sinks=1500)
