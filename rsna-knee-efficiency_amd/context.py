@@ -167,6 +167,30 @@ def _rotary_plan(sections: tuple, base: float) -> bytes:
     return bytes(a)
 
 
+def _may_meet(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether two tensors of one shape and type may have an element in common.  Exact where their strides are the same
+    and nested: then the distance between them must not be a sum of strides times differences of indices."""
+    def span(sizes, strides):
+        return sum((n - 1) * s for n, s in zip(sizes, strides))
+    size, apart = x.element_size(), y.data_ptr() - x.data_ptr()
+    if not -size * span(y.shape, y.stride()) <= apart <= size * span(x.shape, x.stride()):
+        return False
+    if apart % size or x.stride() != y.stride():
+        return True
+    dims = sorted(zip(x.stride(), x.shape), reverse=True)
+
+    def reached(distance: int, at: int) -> bool:
+        if at == len(dims):
+            return distance == 0
+        stride, n = dims[at]
+        rest = span([m for _, m in dims[at + 1:]], [t for t, _ in dims[at + 1:]])
+        if stride == 0:
+            return reached(distance, at + 1)
+        low, high = max(1 - n, -((rest - distance) // stride)), min(n - 1, (distance + rest) // stride)
+        return high - low > 4 or any(reached(distance - i * stride, at + 1) for i in range(low, high + 1))
+    return reached(apart // size, 0)
+
+
 def _rotate(x, positions, sections, base, adjacent, inverse, out):
     _no_tangents(x, positions, out)
     a = hip.RotaryArgs.from_buffer_copy(_rotary_plan(tuple(sections), float(base)))
@@ -182,8 +206,13 @@ def _rotate(x, positions, sections, base, adjacent, inverse, out):
         out = _like(x)
     elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(3) != 1:
         _fail("out must be like x, its channels contiguous")
-    elif out.data_ptr() == x.data_ptr() and out.stride() != x.stride():
-        _fail("out must be x itself, or memory of its own")
+    elif any(s == 0 and n > 1 for n, s in zip(out.shape, out.stride())):
+        _fail("out must not have several elements in one place")
+    elif out.data_ptr() == x.data_ptr():
+        if out.stride() != x.stride():
+            _fail("out must be x itself, or memory of its own")
+    elif x.numel() and _may_meet(x, out):      # (a token's values could be read after another's were written there)
+        x = x.clone(memory_format=torch.contiguous_format)
     if not x.numel():
         return out
     a.x, a.y, a.pos = x.data_ptr(), out.data_ptr(), positions.data_ptr()
@@ -217,7 +246,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, sections, base: float = 100
     sections[a] pairs of channels turn with axis a, pair t of them by positions[..., a] * base^(-t / sections[a]);
     pairs are channels (i, i + pairs), or (2 i, 2 i + 1) when `adjacent`; channels past the pairs are copied.
     positions: (batch, tokens, axes) or, for all of a batch, (tokens, axes).  `inverse` turns back (the gradient; the
-    call is differentiable in x).  `out` may be x itself, where no gradient is asked for.  Queries and keys that lie
+    call is differentiable in x).  `out` may be x itself, where no gradient is asked for, and elements of other places in x's
+    memory (x is then copied first); it must not be expanded.  Queries and keys that lie
     beside each other in one tensor are turned in one call, as x of all their heads."""
     if torch.is_grad_enabled() and x.requires_grad:
         _no_tangents(x, positions, out)
