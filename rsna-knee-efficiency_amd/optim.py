@@ -46,6 +46,9 @@ class AdamW:
         self.device = self.params[0].device
         for p in self.params:
             self._check(p)
+        spans = sorted((p.data_ptr(), p.numel() * p.element_size()) for p in self.params if p.numel())
+        if any(at + size > after for (at, size), (after, _) in zip(spans, spans[1:])):
+            raise ValueError("parameters share memory")      # (two updates of one element would run at once)
         self.lr, self.betas, self.eps, self.weight_decay, self.state_bits = lr, tuple(betas), eps, weight_decay, state_bits
         self.step_count = 0                    # calls of `step`
         # the number of steps of every tensor: one for all as long as none is left out of one, else a list

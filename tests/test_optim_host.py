@@ -63,3 +63,11 @@ def test_every_tensor_counts_its_own_steps(monkeypatch):
         with pytest.raises(ValueError, match="step"):
             opt.load_state_dict(state | bad)
     assert opt.steps == [3] * 4
+
+
+def test_parameters_that_share_memory_are_refused(monkeypatch):
+    flat = torch.zeros(100)
+    for pair in ((flat[:50], flat[49:]), (flat, flat.view(10, 10)), (flat[20:30], flat)):
+        with pytest.raises(ValueError, match="share memory"):
+            _optimizer(monkeypatch, list(pair))
+    _optimizer(monkeypatch, [flat[50:], flat[:50], torch.zeros(0), torch.zeros(0), torch.zeros(3)])
