@@ -106,6 +106,8 @@ class ContextLayer:
             raise ValueError("tokens one at a time need a layer with right = 0")
         if cache.arrived >= cache.k.shape[1]:
             raise ValueError("the cache is full")
+        if x.shape != (cache.k.shape[0], self.width):
+            raise ValueError("x must be (the cache's batch, width)")
         x = x.to(self.dtype)[:, None]
         q, k, v = self._project(x, positions[:, None])
         cache.k[:, cache.arrived], cache.v[:, cache.arrived] = k[:, 0], v[:, 0]
