@@ -44,6 +44,10 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 template <class T>
 using Frag = T __attribute__((ext_vector_type(8)));
+template <class T>
+constexpr bool NARROW = false;                 // whether P and dS have to be brought into T's range
+template <>
+constexpr bool NARROW<f16> = true;
 typedef Vec<uint16_t, 8> Raw;                  // 8 elements as they lie in memory
 
 DEV f32x16 mfma(Frag<bf16> a, Frag<bf16> b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
@@ -251,7 +255,9 @@ DEV bool any_weight(float sum) { return sum > 0.0f || sum != sum; }
 // queries), so a query's statistics are one value a lane, and P goes from registers into the second product.
 // The running maximum m is raised, and the sums scaled, only where a tile exceeds it by more than 2^RISE (P stays below
 // 2^RISE, harmless in float32 and in both types), which after a row's first tiles is rare.
-constexpr float RISE = 6.0f;
+// float16 holds nothing below 2^-25 and little below 2^-14, and P next to one key that outweighs each of many others is
+// that small: it is formed times 2^NARROW_UP (in its exponent, so at no cost), which leaves the sums' quotient as it is.
+constexpr float RISE = 6.0f, NARROW_UP = 8.0f;
 
 template <class T, int D>
 __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
@@ -340,7 +346,7 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[d][r] *= a;
         }
-        const float mc = m == -INFINITY ? 0.0f : m * c;
+        const float mc = (m == -INFINITY ? 0.0f : m * c) - (NARROW<T> ? NARROW_UP : 0.0f);
         float sum = 0.0f;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -365,7 +371,7 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
     swap32(l, l0, l1);
     l = l0 + l1;
     const bool any = any_weight(l);
-    if (p.lse && lane < 32 && i < p.S) p.lse[((int64_t)b * p.H + h) * p.S + i] = any ? (m * c + log2f(l)) * LN2 : -INFINITY;
+    if (p.lse && lane < 32 && i < p.S) p.lse[((int64_t)b * p.H + h) * p.S + i] = any ? (m * c + (log2f(l) - (NARROW<T> ? NARROW_UP : 0.0f))) * LN2 : -INFINITY;
     store_rows<T, ND>((T*)p.out + (((int64_t)b * p.S + i) * p.H + h) * D, acc, any ? 1.0f / l : 0.0f, i < p.S, lane);
 }
 
@@ -386,11 +392,6 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
 // than sums shared through atomics would take, for results that do not depend on an order.
 // Bound as the forward pass, with the matrix unit busy 0.48 of the time: 2 x 8199 tokens of 16 heads of 128 (4 key heads),
 // 1024 before each, in 514 .. 561 us (0.6 PFLOP/s with the products formed twice; two launches after each other took 700).
-template <class T>
-constexpr bool NARROW = false;                 // whether P and dS are brought into T's range
-template <>
-constexpr bool NARROW<f16> = true;
-
 // Of each tile of 64 rows: the largest |do| and |rowsum(do o)| [B][H][tiles], the largest |v| [B][HK][tiles]
 struct Tops {
     float *g, *r, *v;

@@ -147,3 +147,22 @@ def test_many_first_tokens(dev):
     q, k, v, do = _inputs(dev, 7, 1, 4000, 16, 8, 64, 1e-3)
     _check(q, k, v, do, left=3, right=0, sinks=4000)
     _check(q, k, v, do, left=100, right=0, sinks=1500)
+
+
+@pytest.mark.parametrize("high", [17.4, 18.0, 19.0])
+def test_one_key_above_many(dev, high):
+    """One key outweighs each of 131071 others by e^high, which together have up to 0.4 % of the weight: every value is 1,
+    so out is 1, off by P's rounding of that share, one of the result, and the float32 sums: P v has one addition every
+    16 keys, P one every 64, each off by 2^-23 or 2^-24 of the sum (the matrix unit's need not round to the nearest)."""
+    n = 1 << 17
+    q, k = (torch.zeros((1, n, 1, 64), dtype=torch.float16, device=dev) for _ in range(2))
+    q[..., 0] = 1.0
+    k[:, 0, :, 0] = high
+    v = torch.ones_like(k)
+    out, lse = context.window_attention_forward(q, k, v, None, None, scale=1.0)
+    top = k[0, 0, 0, 0].double().item()
+    share = (n - 1) / (n - 1 + math.exp(top))
+    print(f"share {share:.2e} off by {(out.double() - 1).abs().max().item():.2e}", flush=True)
+    assert ((out.double() - 1).abs() <= U * (1 + share) + 2.0 ** -23 * n / 16 + 2.0 ** -24 * n / 64).all()
+    # (32 more additions in a tile, the logarithm, products)
+    assert ((lse.double() - (top + math.log1p((n - 1) * math.exp(-top)))).abs() <= 2.0 ** -24 * (n / 64 + 64 + 4 * top)).all()
