@@ -513,8 +513,8 @@ int d8s_rotary(const D8sRotaryArgs* a, void* stream);
 /* Attention of S tokens within a window and `sinks` first tokens: key j is visible to query i iff j <= i + right,
  * (j >= i - left or j < sinks) and mask[j] is not 0 (mask 0: all).  A query that sees nothing has zeros, lse -inf
  * and no gradient (zeros and -inf also where every score it sees is -infinity); what lies in rows of masked keys is
- * not used.  q, dout [B][S][H][D], k, v [B][S][HK][D] of dtype
- * (D8S_BF16 or D8S_F16; D 64 or 128; H a multiple of HK, query head h uses key head h / (H / HK)) with the given
+ * not used.  q, dout [B][S][H][D], k, v [B][S][HK][D] of dtype (D8S_BF16 or D8S_F16; D 64 or 128; H a multiple of HK,
+ * query head h uses key head h / (H / HK); scale 2^-100 .. 2^100) with the given
  * strides (elements, the last dimension contiguous); out, dq [B][S][H][D], dk, dv [B][S][HK][D] and lse [B][H][S]
  * (natural logarithm of the sum of exponentials) contiguous.  Products are of 16 bits with float32 sums; P and dS
  * are rounded to dtype between two products (for D8S_F16 the gradients multiply both by powers of two that bring them into

@@ -291,8 +291,8 @@ def _attn_args(q, k, v, left, right, sinks, key_mask, scale):
     if D not in (64, 128):
         _fail("64 or 128 channels a head")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 0 < scale < math.inf:
-        _fail("scale must be positive and finite")
+    if not 2.0 ** -100 <= scale <= 2.0 ** 100:
+        _fail("scale must be positive: 2^-100 .. 2^100")
     q, k, v = _last(q), _last(k), _last(v)
     _on_gpu(q, k, v)
     mask_at, mask_sb = 0, 0
@@ -316,7 +316,8 @@ def window_attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
 
     Token i sees token j iff j <= i + right, and j >= i - left or j < sinks, and key_mask[batch, j] (bool, or uint8
     with 0 for absent).  None: no limit on that side.  A token that sees nothing has zeros.  Strides are free (the
-    channels are copied where they are not contiguous).  scale: 1 / sqrt(channels) unless given.
+    channels are copied where they are not contiguous).  scale: 1 / sqrt(channels) unless given
+    (2^-100 .. 2^100).
 
     -> (out like q, lse (batch, heads, tokens) float32: the logarithm of the sum of exponentials, -inf where nothing
     is seen; None without `statistics`)"""
@@ -401,8 +402,8 @@ def window_attention_token(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         _fail("lengths must be (batch,) int32")
     _on_gpu(q, k_cache, v_cache, lengths)
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 0 < scale < math.inf:
-        _fail("scale must be positive and finite")
+    if not 2.0 ** -100 <= scale <= 2.0 ** 100:
+        _fail("scale must be positive: 2^-100 .. 2^100")
     out = _like(q)
     if not out.numel() or not k_cache.shape[1]:
         return out.zero_()

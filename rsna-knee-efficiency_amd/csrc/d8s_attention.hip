@@ -1072,7 +1072,7 @@ int attn_check(const D8sAttnArgs* a, const char* what) {
     AREQ(a->S <= (1 << 29), "more than 2^29 tokens");
     AREQ((int64_t)a->B * a->H * ((a->S + 127) / 128) < (1 << 24), "too many heads and tokens");
     AREQ(a->left >= 0 && a->right >= 0 && a->sinks >= 0, "left, right and sinks must not be negative");
-    AREQ(a->scale > 0 && a->scale < INFINITY && 1.0f / a->scale < INFINITY, "scale must be positive and finite, and 1 / scale too");
+    AREQ(a->scale >= 0x1p-100f && a->scale <= 0x1p100f, "scale must be 2^-100 .. 2^100 (lse / scale and scale log2(e) are float32)");
     AREQ(a->q && a->k && a->v && a->out, "null pointer");
     return 0;
 }
@@ -1117,7 +1117,7 @@ static int token_check(const D8sTokenArgs* a, const char* what) {
     AREQ(a->B >= 1 && a->S >= 1 && a->H >= 1 && a->HK >= 1 && a->H % a->HK == 0, "bad sizes (H a multiple of HK)");
     AREQ((int64_t)a->B * a->H < (1 << 22), "too many heads");
     AREQ(a->left >= 0 && a->sinks >= 0, "left and sinks must not be negative");
-    AREQ(a->scale > 0 && a->scale < INFINITY && 1.0f / a->scale < INFINITY, "scale must be positive and finite, and 1 / scale too");
+    AREQ(a->scale >= 0x1p-100f && a->scale <= 0x1p100f, "scale must be 2^-100 .. 2^100 (lse / scale and scale log2(e) are float32)");
     return 0;
 }
 
