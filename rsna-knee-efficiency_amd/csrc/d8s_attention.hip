@@ -247,8 +247,9 @@ DEV bool any_weight(float sum) { return sum > 0.0f || sum != sum; }
 // ---- forward --------------------------------------------------------------------------------------
 // Bound by its instructions: a wave's tile of 32 x 64 scores is 162 vector operations (32 exponentials among them) beside 16
 // (D = 64) or 32 (D = 128) products of 32 cycles, and the two overlap only between waves.  Measured: 22528 tokens of 4
-// heads of 64, 1024 neighbours each, 43 us (0.41 PFLOP/s; 32 heads without a mask 0.68); 2 x 8199
-// tokens of 16 heads of 128, 1024 before each, 181 us (0.72 PFLOP/s).  Tiles of 32 keys and more waves: 49 and 216 us.
+// heads of 64, 1024 neighbours each, two keys in eight masked, 38 us (0.47 PFLOP/s; 32 heads without a mask 0.68); 2 x 8199
+// tokens of 16 heads of 128, 1024 before each, 182 us (0.72 PFLOP/s).  (In a long row of passes: after a pause the card's
+// clock is lower, 47 us for the first.)  Tiles of 32 keys and more waves: 49 and 216 us where these were 43 and 185.
 //
 // A workgroup runs 128 queries of a head, 32 a wave, over the tiles of 64 keys they can see; keys and values go
 // through two LDS buffers, the next tile's copies in flight while one is computed.  A wave forms s transposed (keys x
@@ -382,16 +383,17 @@ __global__ __launch_bounds__(NT, (D == 64 ? 3 : 2)) void k_attn(D8sAttnArgs p) {
 // the queries that a workgroup runs over (dk; of a lane's own query for dq) and the largest |v| of the keys follows a power
 // that keeps |dS| below 2^15 (P is 1 at most, 2 with its rounding), and nothing above 2^-28 of that bound is
 // held in fewer bits.  It is in the exponent that P is formed from (for dk partly in v), so a tile costs no operation
-// more: 2 x 8199 tokens of 16 heads of 128, 541 us with it and 535 without.  bfloat16 has float32's range and needs none.  The largest
-// norms of every tile of 64 queries and of 64 keys are left by k_attn_delta; queries that see nothing, keys that are
-// masked and rows that are not finite are left out of them, so that they do not cost the others their bits.
+// more: 2 x 8199 tokens of 16 heads of 128, 541 us with it and 535 without.  bfloat16 has float32's range and needs none.
+// The largest norms of every tile of 64 queries and of 64 keys are left by k_attn_delta; queries that see nothing, keys
+// that are masked and rows that are not finite are left out of them, so that they do not cost the others their bits.
 //
 // k_attn_delta leaves rowsum(do o) of every query.  One launch then runs both kinds of workgroups beside each other:
 // first those of the keys (dk and dv, the longer ones), then those of the queries (dq), which fill the compute units
 // that the keys leave; what either writes the other does not read.  Both form s and dP: two products of seven more
 // than sums shared through atomics would take, for results that do not depend on an order.
-// Bound as the forward pass, with the matrix unit busy 0.48 of the time: 2 x 8199 tokens of 16 heads of 128 (4 key heads),
-// 1024 before each, in 514 .. 561 us (0.6 PFLOP/s with the products formed twice; two launches after each other took 700).
+// Bound as the forward pass, with the matrix unit busy 0.44 of the time: 2 x 8199 tokens of 16 heads of 128 (4 key heads),
+// 1024 before each, in 507 .. 539 us from card to card, float16 (0.6 PFLOP/s with the products formed twice; two launches
+// after each other took 700).
 // Of each tile of 64 rows: the largest |do| and |rowsum(do o)| [B][H][tiles], the largest |v| [B][HK][tiles]
 struct Tops {
     float *g, *r, *v;

@@ -7,8 +7,11 @@
 // All sums are float32; the variance is of the centred values (a second look at the registers), so a large mean
 // costs no digits.  Bound by memory: a row is read once into the registers of the 16 lanes, the wave or the
 // workgroup it is shared between, everything else happens there, and it is written once.  Measured, 98303 rows of 1024
-// bfloat16: forward 81 us (5.0 TB/s; a large copy on this card 5.2), gradients 110 us (5.5 TB/s) and 8 us for the
-// columns' sums.
+// bfloat16: forward 76 us (5.3 TB/s; a large copy on this card 5.2), gradients 111 us (5.4 TB/s) and 8 us for the
+// columns' sums.  That is the best width of 16 bits; others, of 10 to 26 million values: forward 2.4 .. 4.7 TB/s, gradients
+// 1.4 .. 3.5 (2406 x 4877 20 and 49 us, 20000 x 1300 29 and 73, 3000 x 8000 22 and 64), where the last vector is
+// read value by value, few waves are resident (32 values a thread) or the parts of the columns' sums are as large as the
+// rows.  float32: 4.0 .. 5.5 and 2.9 .. 5.0.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -281,7 +284,8 @@ __global__ __launch_bounds__(256) void k_norm_cols(D8sNormArgs p, int parts) {
 int norm_rows(int width) { return width <= 128 ? 16 : width <= 2048 ? 4 : 1; }
 
 // Workgroups of the gradients, each of which leaves a part of the columns' sums: four a compute unit keep enough rows
-// in flight (98303 x 1024 bfloat16: 113 us; two a compute unit 165 us, and 4 us less for the sums)
+// in flight (98303 x 1024 bfloat16: 111 us; two a compute unit 165 us, and 4 us less for the sums).  Measured at that
+// width: of few long rows the parts are as large as the rows themselves (3000 x 8000: 131 of 275 MB)
 int norm_parts(const D8sNormArgs* a) {
     const int64_t per = norm_rows(a->width), all = (a->rows + per - 1) / per;
     return (int)std::min<int64_t>(all, 4 * d8s_host_cu_count());
@@ -338,7 +342,7 @@ int norm_check(const D8sNormArgs* a, const char* what) {
 // which is also the gradient, turns back.  The angle is formed in float64 as a number of turns and its whole turns
 // dropped there (three operations), so any position an int32 holds is as exact as a small one; sine and cosine of
 // the rest are float32.  A thread forms those of V pairs of a token once and applies them to the token's heads.
-// Bound by memory: 49152 tokens of 20 heads of 128 float16 channels in 101 us (5.0 TB/s).
+// Bound by memory: 49152 tokens of 20 heads of 128 float16 channels in 109 us (4.6 TB/s; 101 at best).
 template <class T, bool ADJ>
 __global__ __launch_bounds__(256) void k_rotary(D8sRotaryArgs p, int groups, int turned, int per) {
     constexpr int V = 16 / (int)sizeof(T);
