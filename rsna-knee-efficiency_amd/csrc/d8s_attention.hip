@@ -661,7 +661,8 @@ DEV void dkv_body(const D8sAttnArgs& p, const float* delta, const Tops& tops, fl
 #pragma unroll
         for (int k = 0; k < 3; ++k) tops_of[k] = fmaxf(fmaxf(ls[1][4 * k], ls[1][4 * k + 1]), fmaxf(ls[1][4 * k + 2], ls[1][4 * k + 3]));
         const int e = __builtin_amdgcn_readfirstlane(shift_of(__builtin_fmaf(tops_of[0], tops_of[2], tops_of[1])));
-        const int room = __builtin_amdgcn_readfirstlane(max(0, 15 - __builtin_amdgcn_frexp_expf(tops_of[2])));
+        // (2^15 is the largest power that float16 itself holds)
+        const int room = __builtin_amdgcn_readfirstlane(min(max(0, 15 - __builtin_amdgcn_frexp_expf(tops_of[2])), 15));
         of_p = min(max(e, 0), 14);
         of_v = min(max(e - of_p, -10), room);
         of_p = min(of_p, e - of_v);

@@ -166,3 +166,13 @@ def test_one_key_above_many(dev, high):
     assert ((out.double() - 1).abs() <= U * (1 + share) + 2.0 ** -23 * n / 16 + 2.0 ** -24 * n / 64).all()
     # (32 more additions in a tile, the logarithm, products)
     assert ((lse.double() - (top + math.log1p((n - 1) * math.exp(-top)))).abs() <= 2.0 ** -24 * (n / 64 + 64 + 4 * top)).all()
+
+
+@pytest.mark.parametrize("vs", [1e-2, 1e-4, 0.0])
+@pytest.mark.parametrize("size", [1e-3, 1e-5, 1e-7])
+def test_small_values_and_small_gradients(dev, size, vs):
+    """Gradients whose bound is below 2^-16 with values far below 1, to the smallest that float16 holds, and zeros."""
+    for n, how in ((2, dict(left=0, right=0)), (500, dict(left=None, right=0)), (300, dict(left=20, right=20, sinks=3))):
+        q, k, v, do = _inputs(dev, n, 2, n, 2, 1, 64, size, 3.0, vs)
+        got = _check(q, k, v, do, **how)
+        assert all(t.isfinite().all() for t in got)
