@@ -757,14 +757,20 @@ __global__ __launch_bounds__(NT) void k_cache_even_join(D8sCacheAttnArgs p, Even
 // neighbouring tokens at a time, as the transposed values have them.
 // The scale of a block's values is in the exponent that its weights are formed from, relative to a reference that all sums are in units
 // of: the weights are float16 numbers, so the reference follows the scales where they fall VSPAN times below it or rise above (the sums are then
-// scaled; it stays within 2^80 of the largest scale met, for float32's range).
+// scaled).  It is one for all rows, also for those that do not see the block, so float32 keeps every row's sums only where the scales of the
+// workgroup's blocks are within SPREAD of each other and below HIGH.  Where they are not (only bfloat16 values can be such), blocks are run one by
+// one, their products formed by themselves and added times the scale, in units of 1, or, a row at a time, of 1 / LOWER, as with few rows.
+// (2 x 256 queries over 8192 tokens of 8 key heads of 128: 89 us, and 91 where the scales are apart.  Looking at them first costs a bfloat16
+// call a load and some shuffles: 8192 queries over themselves 566 -> 570, 4096 of 64 channels 105 -> 106.)
 //
 // Bound by its instructions: per 32 x 64 scores a wave issues 32 products of 32 cycles (D = 128) beside 218 vector instructions (32 of
 // them its share of the codes' conversion, at 128 rows 64), and two waves a SIMD overlap them in part: 2 x 256 queries of 32 heads over 22528
 // tokens of 8 key heads 198 .. 206 us, 0.92 .. 0.95 PFLOP/s (a large library product 1.36), the matrix unit 0.45 busy at 2.0 GHz.
 // Tried, no better: crews of four waves a barrier apart, one at its products while the other forms weights (219 us: a lone wave's
 // weights wait for themselves); reads of LDS six products ahead by scheduling groups (204); a barrier for two blocks (192 .. 200).
-constexpr float VSPAN = 16.0f;
+constexpr float VSPAN = 16.0f, SPREAD = 0x1p60f;
+// A block that is full and followed by others, the block that is not full, and one whose scale is too far from the others'
+enum Kind { CODED, RAW, APART };
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 DEV f32x16 mfma(Frag<bf16> a, Frag<bf16> b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
@@ -848,219 +854,291 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : W == 4 ? 3 : 4) void k_cache
         }
     }
     const float cs = p.scale * LOG2E;
-    float m = -INFINITY, l = 0.0f, vref = 0.0f, vinv = 0.0f, vtop = 0.0f;
-    f32x16 acc[ND] = {};
-    // the thread's pieces: piece x of the key tile is channels 8 (e % (D / 8)) of token e / (D / 8), of the value tile tokens
-    // 8 (e % 8) of channel e / 8, with e = x * THREADS + threadIdx.x: 8 codes each, as they lie in memory
-    u32x2 kr[PER], vr[PER];
-    const auto load = [&](int j) __attribute__((always_inline)) {
-        const u32x2* kc = (const u32x2*)((const uint8_t*)c.k_code + (head * nb + j) * BLK * D) + threadIdx.x;
-        const u32x2* vc = (const u32x2*)((const uint8_t*)c.v_code + (head * nb + j) * BLK * D) + threadIdx.x;
-#pragma unroll
-        for (int x = 0; x < PER; ++x) {
-            kr[x] = kc[x * THREADS];
-            vr[x] = vc[x * THREADS];
-        }
-    };
-    // (a thread's pieces lie whole tiles of 16 or 32 rows apart, at one place of the swizzle)
-    constexpr int STEP = THREADS * 16;
-    const uint32_t kput = piece_at<D>(key_row(threadIdx.x / (D / 8)), threadIdx.x % (D / 8)), vput = piece_at<64>(threadIdx.x / 8, threadIdx.x % 8);
-    const auto put1 = [&](u32x4* tile, uint32_t at, const u32x2* codes, int x) __attribute__((always_inline)) {
-        at_byte(tile, at + x * STEP) = __builtin_bit_cast(u32x4, codes_frag<E4M3>(codes[x][0], codes[x][1]));
-    };
-    const auto put = [&](u32x4* tile, uint32_t at, const u32x2* codes) __attribute__((always_inline)) {
-#pragma unroll
-        for (int x = 0; x < PER; ++x) put1(tile, at, codes, x);
-    };
-    // One block in LDS, of type C: scores times by, the values' scale vs.  Where NEXT, the next block's codes go to nk and nv on the
-    // way, their conversions between the products, which leave most of the issue slots.  (Waves whose rows see nothing of a block run it all the
-    // same: a way round it cost copies of the sums in every block.)
-    const auto turn = [&](auto type, auto has_next, const auto& qf, u32x4* tk, u32x4* tv, u32x4* nk, u32x4* nv, int k0, float by,
-                          float vs) __attribute__((always_inline)) {
-        typedef decltype(type) C;
-        constexpr bool NEXT = decltype(has_next)::value;
-        const uint32_t ka = fresh(piece_at<D>(lane % 32, half)), va = fresh(piece_at<64>(lane % 32, half));
-        f32x16 s[2];
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-                s[u] = mfma(__builtin_bit_cast(Frag<C>, at_byte(tk, (ka ^ (k << 5)) + u * 64 * D)), qf[k], k == 0 ? f32x16{} : s[u]);
-            if constexpr (NEXT)
-                if (k % (KS / PER) == KS / PER - 1) {
-                    fence();
-                    put1(nk, kput, kr, k / (KS / PER));
-                    fence();
-                }
-        }
-        by = by == 0.0f ? 0x1p-126f : by;      // (scores of a block of zeros are zeros; masked ones stay -infinity)
-        // the reference of the values' scales (0 at first; a block of zeros needs none)
-        // (The last block's weights are bfloat16 numbers where its values are, whose range needs no reference of these: it is 1, or 1 / LOWER
-        // where the values, or those met before, ask for it.)
-        constexpr bool RAW = !NEXT && __is_same(C, bf16);
-        float turned = 1.0f;
-        if (RAW ? vref != vs : (vs > 0.0f) & ((vs > vref * 2.0f) | (vs * VSPAN < vref))) {
-            vtop = fmaxf(vtop, vs);
-            const float to = RAW ? vs : fmaxf(fmaxf(vs, vtop * 0x1p-80f), 0x1p-126f);
-            turned = vref / to;
-            vref = to;
-            vinv = 1.0f / to;
-        }
-        float ratio = RAW ? vinv : vs == 0.0f ? 1.0f : vs * vinv;
-        if (!RAW) ratio = ratio < 0x1p-16f ? 0x1p-16f : ratio;       // (of a scale 2^-80 of the largest: its values are nothing beside that one's)
-        float lift = __builtin_amdgcn_logf(ratio) + NARROW_UP, weigh = __builtin_amdgcn_rcpf(ratio);
-        if (!(k0 + BLK <= n && k0 + BLK - 1 <= wlo + p.right && (k0 >= whi - p.left || k0 + BLK <= p.sinks))) {
-            uint64_t vis = 0;
-            if (on) vis = bits_below(min(i + p.right, n - 1) + 1 - k0) & (~bits_below(i - p.left - k0) | bits_below(p.sinks - k0));
-            // (rows that see nothing of the block do not meet a scale of it that is not a number)
-            by = vis ? by : 1.0f;
-            lift = vis ? lift : 0.0f;
-            weigh = vis ? weigh : 1.0f;
-            const uint32_t mine[2] = {(uint32_t)(vis >> (8 * half)), (uint32_t)(vis >> (32 + 8 * half))};
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    // (register x of s[u] is token 32 u + 16 (x / 8) + 8 half + x % 8)
-                    const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe((int)mine[u], 16 * (x / 8) + x % 8, 1);
-                    s[u][x] = __uint_as_float((__float_as_uint(s[u][x]) & keep) | (0xff800000u & ~keep));
-                }
-        }
-        float top = s[0][0];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int x = 0; x < 16; ++x) top = fmaxf(top, s[u][x]);
-        float t0, t1;
-        swap32(top, t0, t1);
-        top = fmaxf(t0, t1) * by;
-        if (__any((top > m + RISE) | (turned != 1.0f))) {
-            const float up = fmaxf(m, top), a = up == -INFINITY ? 1.0f : exp2_(m - up);
-            m = up;
-            l *= a;
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int x = 0; x < 16; ++x) acc[d][x] *= a * turned;
-        }
-        const float base = (m == -INFINITY ? 0.0f : m) - lift;
-        float sum = 0.0f;
-        const auto weight = [&](int u, int x) __attribute__((always_inline)) {
-            s[u][x] = exp2_(__builtin_fmaf(s[u][x], by, -base));
-        };
-        const auto summed = [&](int u, int x) __attribute__((always_inline)) {
-            float z[4];
-#pragma unroll
-            for (int y = 0; y < 4; ++y) z[y] = s[u][x + y] + s[u][x + 4 + y];
-            sum += (z[0] + z[1]) + (z[2] + z[3]);
-        };
-        const auto product = [&](int k) __attribute__((always_inline)) {
-            Frag<C> w;
-#pragma unroll
-            for (int x = 0; x < 8; ++x) w[x] = (C)s[k / 2][8 * (k % 2) + x];
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-                acc[d] = mfma(__builtin_bit_cast(Frag<C>, at_byte(tv, (va ^ (k << 5)) + d * 32 * 2 * BLK)), w, acc[d]);
-        };
-#pragma unroll
-        for (int x = 0; x < 8; ++x) weight(0, x);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            fence();
-            product(k);
-            fence();
-            summed(k / 2, 8 * (k % 2));
-            if (k < 3) {
-#pragma unroll
-                for (int x = 0; x < 8; ++x) weight((k + 1) / 2, 8 * ((k + 1) % 2) + x);
-            }
-            if constexpr (NEXT)
-                if (k % (4 / PER) == 4 / PER - 1) put1(nv, vput, vr, k / (4 / PER));
-        }
-        l = __builtin_fmaf(sum, weigh, l);
-    };
     // the block that is not full is the last one, if it is among the share's
     const int full = n / BLK;
     const int coded = e1 > e0 && list.at(e1 - 1) >= full ? e1 - 1 : e1;
-    if (e0 < coded) {
-        load(list.at(e0));
-        put(lk0, kput, kr);
-        put(lv0, vput, vr);
-        load(list.at(min(e0 + 1, coded - 1)));
-    }
-    const auto step = [&](int e, u32x4* tk, u32x4* tv, u32x4* nk, u32x4* nv) __attribute__((always_inline)) {
-        const int j = list.at(e);
-        __syncthreads();                       // the block is there, and the other one is no longer read
-        turn(f16(), std::true_type(), q, tk, tv, nk, nv, j * BLK, ldexpf(cs * c.k_scale[head * nb + j], -down), c.v_scale[head * nb + j]);
-        load(list.at(min(e + 2, coded - 1)));  // (past the last block the same again, into the buffer that is not read)
-    };
-    for (int e = e0; e < coded; e += 2) {
-        step(e, lk0, lv0, lk1, lv1);
-        if (e + 1 < coded) step(e + 1, lk1, lv1, lk0, lv0);
-    }
-    if (coded < e1) {                          // the tail, in its own type
-        __syncthreads();
-        bool high = false;
-        const Raw* kt = (const Raw*)((const uint16_t*)c.k_tail + head * BLK * D);
-        const Raw* vt = (const Raw*)((const uint16_t*)c.v_tail + head * BLK * D);
-#pragma unroll
-        for (int x = 0; x < PER; ++x) {
-            const int e = x * THREADS + threadIdx.x, there = n - full * BLK - 8 * (e % 8);     // of the piece's 8 tokens; the others are not used
-            at_byte(lk0, kput + x * STEP) = __builtin_bit_cast(u32x4, kt[e]);
-            Raw v = vt[e];
-#pragma unroll
-            for (int y = 0; y < 8; ++y) v[y] = y < there ? v[y] : 0;
-            const u32x4 words = at_byte(lv0, vput + x * STEP) = __builtin_bit_cast(u32x4, v);
-            if constexpr (__is_same(T, bf16))
-#pragma unroll
-                for (int y = 0; y < 4; ++y) high |= high_values(words[y]);
+    constexpr bool WIDE = __is_same(T, bf16);
+    bool apart = false;                        // the scales of the values are too far from each other
+    if constexpr (WIDE) {
+        float least = INFINITY, most = 0.0f;
+        for (int e = e0 + lane; e < coded; e += 64) {
+            const float vs = c.v_scale[head * nb + list.at(e)];
+            least = vs > 0.0f ? fminf(least, vs) : least;
+            most = fmaxf(most, vs);
         }
-        int* waves = (int*)lk1;                // (not read any more)
-        const bool wave_high = __any(high);
-        if (lane == 0) waves[wave] = wave_high;
-        __syncthreads();
-        high = false;
 #pragma unroll
-        for (int x = 0; x < W; ++x) high |= waves[x] != 0;
-        high &= on && min(i + p.right, n - 1) >= full * BLK;         // (a row at a time, as above)
-        const bool lower = __is_same(T, bf16) && (high || vref > 1.0f / LOWER);
-        Frag<T> x[KS];
-#pragma unroll
-        for (int k = 0; k < KS; ++k) x[k] = __builtin_bit_cast(Frag<T>, *(const Raw*)(qp + 16 * k + 8 * half));
-        turn(T(), std::false_type(), x, lk0, lv0, lk0, lv0, full * BLK, cs, lower ? 1.0f / LOWER : 1.0f);
+        for (int o = 8; o >= 1; o /= 2) least = fminf(least, __shfl_xor(least, o));
+        float x, y;
+        swap16(least, x, y);
+        swap32(fminf(x, y), x, y);
+        least = fminf(x, y);
+        apart = __any(most > HIGH || most > least * SPREAD);
     }
-    float l0, l1;
-    swap32(l, l0, l1);
-    l = l0 + l1;
-    if (r >= rows) return;
-    const int64_t at = ((int64_t)b * p.T + t) * p.H + h;
-    const bool any = on && any_weight(l);
-    const float each = 1.0f / l;
-    if (split == 1) {
-        T* o = (T*)p.out + at * D + 4 * half;
+    const auto job = [&](auto far) __attribute__((always_inline)) {
+        constexpr bool FAR = decltype(far)::value;
+        float m = -INFINITY, l = 0.0f, vref = FAR ? 1.0f : 0.0f, vinv = 0.0f, low = 1.0f;          // (sums are in units of vref / low, low a row's own)
+        f32x16 acc[ND] = {};
+        // the thread's pieces: piece x of the key tile is channels 8 (e % (D / 8)) of token e / (D / 8), of the value tile tokens
+        // 8 (e % 8) of channel e / 8, with e = x * THREADS + threadIdx.x: 8 codes each, as they lie in memory
+        u32x2 kr[PER], vr[PER];
+        const auto load = [&](int j) __attribute__((always_inline)) {
+            const u32x2* kc = (const u32x2*)((const uint8_t*)c.k_code + (head * nb + j) * BLK * D) + threadIdx.x;
+            const u32x2* vc = (const u32x2*)((const uint8_t*)c.v_code + (head * nb + j) * BLK * D) + threadIdx.x;
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int x = 0; x < 16; x += 4) {
-                float f[4];
-#pragma unroll
-                for (int y = 0; y < 4; ++y) f[y] = any ? acc[d][x + y] * each * vref : 0.0f;
-                store_n<T, 4>(o + 32 * d + 2 * x, 4, f);
+            for (int x = 0; x < PER; ++x) {
+                kr[x] = kc[x * THREADS];
+                vr[x] = vc[x * THREADS];
             }
-    } else {
-        const Part z{part, split, (int64_t)c.B * p.T * p.H};
-        if (half == 0) *z.template stats<D>(cut, at) = u32x2{__float_as_uint(on ? m : -INFINITY), __float_as_uint(on ? l : 0.0f)};
-        float* o = z.template sums<D>(cut, at) + 4 * half;
+        };
+        // (a thread's pieces lie whole tiles of 16 or 32 rows apart, at one place of the swizzle)
+        constexpr int STEP = THREADS * 16;
+        const uint32_t kput = piece_at<D>(key_row(threadIdx.x / (D / 8)), threadIdx.x % (D / 8)), vput = piece_at<64>(threadIdx.x / 8, threadIdx.x % 8);
+        const auto put1 = [&](u32x4* tile, uint32_t at, const u32x2* codes, int x) __attribute__((always_inline)) {
+            at_byte(tile, at + x * STEP) = __builtin_bit_cast(u32x4, codes_frag<E4M3>(codes[x][0], codes[x][1]));
+        };
+        const auto put = [&](u32x4* tile, uint32_t at, const u32x2* codes) __attribute__((always_inline)) {
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
+            for (int x = 0; x < PER; ++x) put1(tile, at, codes, x);
+        };
+        // One block in LDS: scores times by, the values' scale vs; `high`: which tokens have values above 1 / LOWER.  Of CODED ones
+        // the next block's codes go to nk and nv on the way, their conversions between the products, which leave most of the issue slots.
+        // (Waves whose rows see nothing of a block run it all the same: a way round it cost copies of the sums in every block.)
+        const auto turn = [&](auto kind, const auto& qf, u32x4* tk, u32x4* tv, u32x4* nk, u32x4* nv, int k0, float by, float vs,
+                              uint64_t high) __attribute__((always_inline)) {
+            constexpr Kind KIND = decltype(kind)::value;
+            typedef std::conditional_t<KIND == RAW, T, f16> C;
+            constexpr bool NEXT = KIND == CODED;
+            const uint32_t ka = fresh(piece_at<D>(lane % 32, half)), va = fresh(piece_at<64>(lane % 32, half));
+            f32x16 s[2];
 #pragma unroll
-            for (int x = 0; x < 16; x += 4) {
-                f32x4 f;
+            for (int k = 0; k < KS; ++k) {
 #pragma unroll
-                for (int y = 0; y < 4; ++y) f[y] = any ? acc[d][x + y] * each * vref : 0.0f;
-                *(f32x4*)(o + 32 * d + 2 * x) = f;
+                for (int u = 0; u < 2; ++u)
+                    s[u] = mfma(__builtin_bit_cast(Frag<C>, at_byte(tk, (ka ^ (k << 5)) + u * 64 * D)), qf[k], k == 0 ? f32x16{} : s[u]);
+                if constexpr (NEXT)
+                    if (k % (KS / PER) == KS / PER - 1) {
+                        fence();
+                        put1(nk, kput, kr, k / (KS / PER));
+                        fence();
+                    }
             }
-    }
+            by = by == 0.0f ? 0x1p-126f : by;      // (scores of a block of zeros are zeros; masked ones stay -infinity)
+            // the reference of the values' scales (0 at first; a block of zeros needs none), 1 for blocks that need none of these
+            float turned = 1.0f, ratio = 1.0f;
+            if constexpr (KIND == CODED || !WIDE) {
+                if ((vs > 0.0f) & ((vs > vref * 2.0f) | (vs * VSPAN < vref))) {
+                    const float to = fmaxf(vs, 0x1p-126f);
+                    turned = vref / to;
+                    vref = to;
+                    vinv = 1.0f / to;
+                }
+                ratio = vs == 0.0f ? 1.0f : vs * vinv;
+            } else if (!FAR) {
+                turned = vref;
+                vref = 1.0f;
+            }
+            float lift = __builtin_amdgcn_logf(ratio) + NARROW_UP, weigh = __builtin_amdgcn_rcpf(ratio);
+            uint64_t seen = on ? ~0ull : 0;        // tokens of the block that the row sees
+            if (!(k0 + BLK <= n && k0 + BLK - 1 <= wlo + p.right && (k0 >= whi - p.left || k0 + BLK <= p.sinks))) {
+                uint64_t vis = 0;
+                if (on) vis = bits_below(min(i + p.right, n - 1) + 1 - k0) & (~bits_below(i - p.left - k0) | bits_below(p.sinks - k0));
+                // (rows that see nothing of the block do not meet a scale of it that is not a number)
+                by = vis ? by : 1.0f;
+                lift = vis ? lift : 0.0f;
+                weigh = vis ? weigh : 1.0f;
+                seen = vis;
+                const uint32_t mine[2] = {(uint32_t)(vis >> (8 * half)), (uint32_t)(vis >> (32 + 8 * half))};
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        // (register x of s[u] is token 32 u + 16 (x / 8) + 8 half + x % 8)
+                        const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe((int)mine[u], 16 * (x / 8) + x % 8, 1);
+                        s[u][x] = __uint_as_float((__float_as_uint(s[u][x]) & keep) | (0xff800000u & ~keep));
+                    }
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) top = fmaxf(top, s[u][x]);
+            float t0, t1;
+            swap32(top, t0, t1);
+            top = fmaxf(t0, t1) * by;
+            if constexpr (KIND != CODED && WIDE) {
+                // (a row at a time: one that does not see such values may have ones that would not be left of it)
+                const bool lower = (high & seen) && low == 1.0f;
+                turned *= lower ? LOWER : 1.0f;
+                low = lower ? LOWER : low;
+                if (KIND == RAW) {                 // bfloat16 weights take the unit themselves
+                    lift = low == 1.0f ? NARROW_UP : NARROW_UP - 64.0f;
+                    weigh = 1.0f / low;
+                }
+            }
+            if (__any((top > m + RISE) | (turned != 1.0f))) {
+                const float up = fmaxf(m, top), a = up == -INFINITY ? 1.0f : exp2_(m - up);
+                m = up;
+                l *= a;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) acc[d][x] *= a * turned;
+            }
+            const float base = (m == -INFINITY ? 0.0f : m) - lift;
+            float sum = 0.0f;
+            const auto weight = [&](int u, int x) __attribute__((always_inline)) {
+                s[u][x] = exp2_(__builtin_fmaf(s[u][x], by, -base));
+            };
+            const auto summed = [&](int u, int x) __attribute__((always_inline)) {
+                float z[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) z[y] = s[u][x + y] + s[u][x + 4 + y];
+                sum += (z[0] + z[1]) + (z[2] + z[3]);
+            };
+            const auto weights = [&](int k) __attribute__((always_inline)) {
+                Frag<C> w;
+#pragma unroll
+                for (int x = 0; x < 8; ++x) w[x] = (C)s[k / 2][8 * (k % 2) + x];
+                return w;
+            };
+            const auto values = [&](int k, int d) __attribute__((always_inline)) {
+                return __builtin_bit_cast(Frag<C>, at_byte(tv, (va ^ (k << 5)) + d * 32 * 2 * BLK));
+            };
+            if constexpr (KIND == APART) {
+                Frag<C> w[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) weight(k / 2, 8 * (k % 2) + x);
+                    summed(k / 2, 8 * (k % 2));
+                    w[k] = weights(k);
+                }
+                const float scale = seen ? vs * low : 0.0f;    // (also one that is not a number)
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    f32x16 o = {};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o = mfma(values(k, d), w[k], o);
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) acc[d][x] = __builtin_fmaf(o[x], scale, acc[d][x]);
+                }
+            } else {
+#pragma unroll
+                for (int x = 0; x < 8; ++x) weight(0, x);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    fence();
+                    const Frag<C> w = weights(k);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) acc[d] = mfma(values(k, d), w, acc[d]);
+                    fence();
+                    summed(k / 2, 8 * (k % 2));
+                    if (k < 3) {
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) weight((k + 1) / 2, 8 * ((k + 1) % 2) + x);
+                    }
+                    if constexpr (NEXT)
+                        if (k % (4 / PER) == 4 / PER - 1) put1(nv, vput, vr, k / (4 / PER));
+                }
+            }
+            l = __builtin_fmaf(sum, weigh, l);
+        };
+        const auto by_of = [&](int j) __attribute__((always_inline)) { return ldexpf(cs * c.k_scale[head * nb + j], -down); };
+        if constexpr (FAR) {
+#pragma unroll 1
+            for (int e = e0; e < coded; ++e) {
+                const int j = list.at(e);
+                const float vs = c.v_scale[head * nb + j];
+                load(j);
+                __syncthreads();                   // the tiles are no longer read
+                put(lk0, kput, kr);
+                put(lv0, vput, vr);
+                __syncthreads();
+                turn(std::integral_constant<Kind, APART>(), q, lk0, lv0, lk0, lv0, j * BLK, by_of(j), vs, vs > HIGH ? ~0ull : 0);
+            }
+        } else {
+            if (e0 < coded) {
+                load(list.at(e0));
+                put(lk0, kput, kr);
+                put(lv0, vput, vr);
+                load(list.at(min(e0 + 1, coded - 1)));
+            }
+            const auto step = [&](int e, u32x4* tk, u32x4* tv, u32x4* nk, u32x4* nv) __attribute__((always_inline)) {
+                const int j = list.at(e);
+                __syncthreads();                   // the block is there, and the other one is no longer read
+                turn(std::integral_constant<Kind, CODED>(), q, tk, tv, nk, nv, j * BLK, by_of(j), c.v_scale[head * nb + j], 0);
+                load(list.at(min(e + 2, coded - 1)));          // (past the last block the same again, into the buffer that is not read)
+            };
+            for (int e = e0; e < coded; e += 2) {
+                step(e, lk0, lv0, lk1, lv1);
+                if (e + 1 < coded) step(e + 1, lk1, lv1, lk0, lv0);
+            }
+        }
+        if (coded < e1) {                          // the tail, in its own type
+            __syncthreads();
+            bool high = false;
+            const Raw* kt = (const Raw*)((const uint16_t*)c.k_tail + head * BLK * D);
+            const Raw* vt = (const Raw*)((const uint16_t*)c.v_tail + head * BLK * D);
+#pragma unroll
+            for (int x = 0; x < PER; ++x) {
+                const int e = x * THREADS + threadIdx.x, there = n - full * BLK - 8 * (e % 8);     // of the piece's 8 tokens; the others are not used
+                at_byte(lk0, kput + x * STEP) = __builtin_bit_cast(u32x4, kt[e]);
+                Raw v = vt[e];
+#pragma unroll
+                for (int y = 0; y < 8; ++y) v[y] = y < there ? v[y] : 0;
+                const u32x4 words = at_byte(lv0, vput + x * STEP) = __builtin_bit_cast(u32x4, v);
+                if constexpr (__is_same(T, bf16))
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) high |= high_values(words[y]);
+            }
+            int* waves = (int*)lk1;                // (not read any more)
+            const bool wave_high = __any(high);
+            if (lane == 0) waves[wave] = wave_high;
+            __syncthreads();
+            high = false;
+#pragma unroll
+            for (int x = 0; x < W; ++x) high |= waves[x] != 0;
+            Frag<T> x[KS];
+#pragma unroll
+            for (int k = 0; k < KS; ++k) x[k] = __builtin_bit_cast(Frag<T>, *(const Raw*)(qp + 16 * k + 8 * half));
+            turn(std::integral_constant<Kind, RAW>(), x, lk0, lv0, lk0, lv0, full * BLK, cs, 1.0f, high ? ~0ull : 0);
+        }
+        float l0, l1;
+        swap32(l, l0, l1);
+        l = l0 + l1;
+        if (r >= rows) return;
+        const int64_t at = ((int64_t)b * p.T + t) * p.H + h;
+        const bool any = on && any_weight(l);
+        const float each = 1.0f / l, unit = vref * (1.0f / low);
+        if (split == 1) {
+            T* o = (T*)p.out + at * D + 4 * half;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int x = 0; x < 16; x += 4) {
+                    float f[4];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) f[y] = any ? acc[d][x + y] * each * unit : 0.0f;
+                    store_n<T, 4>(o + 32 * d + 2 * x, 4, f);
+                }
+        } else {
+            const Part z{part, split, (int64_t)c.B * p.T * p.H};
+            if (half == 0) *z.template stats<D>(cut, at) = u32x2{__float_as_uint(on ? m : -INFINITY), __float_as_uint(on ? l : 0.0f)};
+            float* o = z.template sums<D>(cut, at) + 4 * half;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int x = 0; x < 16; x += 4) {
+                    f32x4 f;
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) f[y] = any ? acc[d][x + y] * each * unit : 0.0f;
+                    *(f32x4*)(o + 32 * d + 2 * x) = f;
+                }
+        }
+    };
+    // (a loop of its own: a way between the two in one loop cost copies of the sums in every block)
+    if (WIDE && apart) job(std::true_type());
+    else job(std::false_type());
 }
 
 // A row's shares joined, four channels a thread.  With few rows K threads share its channels, each some of the shares.
