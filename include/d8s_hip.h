@@ -613,7 +613,7 @@ int d8s_cache_read(const D8sCacheReadArgs* a, void* stream);
  * HK (query head h uses key head h / (H / HK)); out [B][T][H][D] contiguous: zeros for a query that sees nothing, that is
  * past its row's count, or whose position would be negative.  scale 2^-100 .. 2^100.  Scores and sums are float32, with the scales
  * of the codes in them; the weights are rounded to float16 (in the last, 16-bit block to dtype) between the two products.
- * A query's sums are of the keys that it sees alone; where those have bfloat16 values above 2^64 (of a block: any of its
+ * A query's sums are of the keys that it sees alone; where those have bfloat16 values above 2^64 (of a full block: any of its
  * values, if it sees one of its keys) they are held in units of 2^64, so what others below 2^-70 add to them loses digits.
  * Equal inputs give equal bits.  `workspace`: device memory of d8s_cache_attention_workspace bytes (may be 0), 16-byte aligned. */
 typedef struct D8sCacheAttnArgs {

@@ -298,8 +298,15 @@ constexpr float RISE = 6.0f, NARROW_UP = 8.0f;
 // Weights are up to 2^(NARROW_UP + RISE), and bfloat16 values up to float32's own limit: once values (of a scale) above 2^64 (HIGH) are met,
 // sums are held times LOWER.  Parts of a row are left as means of values, which stay in range, with the sum of their weights.
 constexpr float LOWER = 0x1p-64f, HIGH = 0x1p56f;
-// Whether one of two bfloat16 numbers is 2^64 or more, or none
-DEV bool high_values(uint32_t two) { return ((two & 0x7fff7fffu) + 0x20802080u) & 0x80008000u; }
+// Bits 15 and 31: whether the first and the second of two bfloat16 numbers is 2^64 or more, or none
+DEV uint32_t high_values(uint32_t two) { return ((two & 0x7fff7fffu) + 0x20802080u) & 0x80008000u; }
+// Of four such pairs a bit each, the first in the lowest
+DEV uint32_t high_bits(const uint32_t* two) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) bits |= (two[y] >> 15 & 1) << (2 * y) | (two[y] >> 31) << (2 * y + 1);
+    return bits;
+}
 
 DEV f32x4 mfma(Frag<bf16> a, Frag<bf16> b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 DEV f32x4 mfma(Frag<f16> a, Frag<f16> b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -576,7 +583,7 @@ DEV void rows_job(const D8sCacheAttnArgs& p, const Rows& a, int rt, int hk, int 
         const uint64_t vis = visible(full * BLK);
         weights(s, cs, vis);
         const int there = n - full * BLK - 16 * g;          // of the lane's 16 tokens; what lies past them is not used
-        bool high = false;
+        uint32_t two[8] = {};                  // which of the lane's 16 tokens have high values
 #pragma unroll
         for (int d = 0; d < VL; ++d)
 #pragma unroll
@@ -587,9 +594,17 @@ DEV void rows_job(const D8sCacheAttnArgs& p, const Rows& a, int rt, int hk, int 
                 vw[2 * d + k] = __builtin_bit_cast(u32x4, v);
                 if constexpr (__is_same(T, bf16))
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) high |= high_values(vw[2 * d + k][x]);
+                    for (int x = 0; x < 4; ++x) two[4 * k + x] |= high_values(vw[2 * d + k][x]);
             }
-        lower(__any(high) && vis);
+        uint32_t high = high_bits(two) | high_bits(two + 4) << 8;
+        if (__any(high)) {
+#pragma unroll
+            for (int o = 1; o < 16; o *= 2) high |= (uint32_t)__shfl_xor((int)high, o);
+            uint64_t all = 0;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) all |= (uint64_t)(uint32_t)__shfl((int)high, 16 * x) << (16 * x);
+            lower(all & vis);
+        }
         Frag<T> w[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -1076,7 +1091,7 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : W == 4 ? 3 : 4) void k_cache
         }
         if (coded < e1) {                          // the tail, in its own type
             __syncthreads();
-            bool high = false;
+            uint32_t two[4] = {};                  // which of the thread's 8 tokens have high values
             const Raw* kt = (const Raw*)((const uint16_t*)c.k_tail + head * BLK * D);
             const Raw* vt = (const Raw*)((const uint16_t*)c.v_tail + head * BLK * D);
 #pragma unroll
@@ -1089,19 +1104,24 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : W == 4 ? 3 : 4) void k_cache
                 const u32x4 words = at_byte(lv0, vput + x * STEP) = __builtin_bit_cast(u32x4, v);
                 if constexpr (__is_same(T, bf16))
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) high |= high_values(words[y]);
+                    for (int y = 0; y < 4; ++y) two[y] |= high_values(words[y]);
             }
-            int* waves = (int*)lk1;                // (not read any more)
-            const bool wave_high = __any(high);
-            if (lane == 0) waves[wave] = wave_high;
-            __syncthreads();
-            high = false;
+            uint64_t high = 0;
+            if constexpr (WIDE) {
+                // (lanes l and l + 8 have the same tokens)
+                uint32_t bits = high_bits(two);
 #pragma unroll
-            for (int x = 0; x < W; ++x) high |= waves[x] != 0;
+                for (int o = 8; o < 64; o *= 2) bits |= (uint32_t)__shfl_xor((int)bits, o);
+                if (lane < 8) ((uint8_t*)lk1)[8 * wave + lane] = (uint8_t)bits;        // (not read any more)
+            }
+            __syncthreads();
+            if constexpr (WIDE)
+#pragma unroll
+                for (int x = 0; x < W; ++x) high |= ((const uint64_t*)lk1)[x];
             Frag<T> x[KS];
 #pragma unroll
             for (int k = 0; k < KS; ++k) x[k] = __builtin_bit_cast(Frag<T>, *(const Raw*)(qp + 16 * k + 8 * half));
-            turn(std::integral_constant<Kind, RAW>(), x, lk0, lv0, lk0, lv0, full * BLK, cs, 1.0f, high ? ~0ull : 0);
+            turn(std::integral_constant<Kind, RAW>(), x, lk0, lv0, lk0, lv0, full * BLK, cs, 1.0f, high);
         }
         float l0, l1;
         swap32(l, l0, l1);

@@ -155,7 +155,7 @@ def cached_attention(q: torch.Tensor, cache: QuantizedCache, left: int | None = 
     The token at position i of its row sees token j iff j <= i + right, and j >= i - left or j < sinks (None: no limit on that
     side): as in `context.window_attention` over all of the row.  -> out like q: zeros for a query that sees nothing or is past
     its row's count.  scale: 1 / sqrt(channels) unless given (2^-100 .. 2^100).  (A value of the last, 16-bit block that is not
-    finite can spoil the queries beside those that see it.  A query that sees bfloat16 values above 2^64, or some token of a
+    finite can spoil the queries beside those that see it.  A query that sees bfloat16 values above 2^64, or some token of a full
     block that has one, loses digits of what others below 2^-70 add to its result.)"""
     _no_gradients(q)
     if q.dim() != 4 or q.shape[0] != cache.batch or q.shape[3] != cache.channels or q.shape[2] < 1 or q.shape[2] % cache.key_heads:

@@ -110,3 +110,22 @@ def test_values_whose_weights_are_zero(dev, codes, new, h, hk):
             cache = QuantizedCache(1, n, hk, d, codes, BF16, dev)
             cache.append(k.to(BF16), v.to(BF16))
             _check(cache, q.to(BF16))
+
+
+@pytest.mark.parametrize("batch,new,h,hk", [(1, 2500, 16, 4), (1, 700, 64, 2), (1, 45, 4, 2), (3, 2, 8, 2)])
+@pytest.mark.parametrize("codes,d", [(INT8, 128), (E4M3, 64)])
+def test_tokens_of_the_last_block_that_a_row_does_not_see(dev, codes, d, batch, new, h, hk):
+    """Large values of single tokens of the last block, the others far below: queries before such a token keep all of theirs."""
+    g, n = torch.Generator(device=dev).manual_seed(new), 3000           # 56 tokens in the last block
+    q, k = (torch.randn((batch, t, heads, d), generator=g, device=dev).to(BF16) for t, heads in ((new, h), (n, hk)))
+    unit = torch.rand((batch, n, hk, d), generator=g, device=dev).double() * 2 - 1
+    for at in ([n - 1], [n - 20], [n - 56], [n - 50, n - 9]):
+        for small in (0.0, -66.0, -100.0):
+            print(f"last block {at} 2^{small} {codes} new={new}", flush=True)
+            v = unit * 2.0 ** small
+            v[:, at, 0, 5] = 2.0 ** 127
+            v[:, at, hk - 1, d - 1] = -(2.0 ** 64)
+            cache = QuantizedCache(batch, n + 40, hk, d, codes, BF16, dev)
+            cache.append(k, v.to(BF16))
+            _check(cache, q)
+            _check(cache, q, 40, 3, 2)
