@@ -330,6 +330,14 @@ DEV Frag<f16> codes_frag(uint32_t lo, uint32_t hi) {
     return Frag<f16>{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
 }
 
+// What a block's scores are times: the scale (with log2(e)), the scale of its keys, and for bfloat16 rows 2^-down.  The powers of two of the
+// first and the last are joined and taken by the second, exactly: no product leaves float32 that the result does not.
+template <class T>
+DEV float unit_of(float scale, float keys, int down) {
+    if constexpr (!__is_same(T, bf16)) return scale * keys;
+    return ldexpf(keys, __builtin_amdgcn_frexp_expf(scale) - 1 - down) * (2.0f * __builtin_amdgcn_frexp_mantf(scale));
+}
+
 // Bits 0 .. 63 below n (any n)
 DEV uint64_t bits_below(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : ~(~0ull << n); }
 
@@ -541,7 +549,7 @@ DEV void rows_job(const D8sCacheAttnArgs& p, const Rows& a, int rt, int hk, int 
                 s[u] = mfma(codes_frag<E4M3>(w[k % 2 * 2], w[k % 2 * 2 + 1]), q[k], s[u]);
             }
         }
-        const float by = ldexpf(cs * ks, -down);
+        const float by = unit_of<T>(cs, ks, down);
         load_k(next);
         const uint64_t vis = visible(j * BLK);
         weights(s, by, vis);
@@ -1058,7 +1066,7 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : W == 4 ? 3 : 4) void k_cache
             }
             l = __builtin_fmaf(sum, weigh, l);
         };
-        const auto by_of = [&](int j) __attribute__((always_inline)) { return ldexpf(cs * c.k_scale[head * nb + j], -down); };
+        const auto by_of = [&](int j) __attribute__((always_inline)) { return unit_of<T>(cs, c.k_scale[head * nb + j], down); };
         if constexpr (FAR) {
 #pragma unroll 1
             for (int e = e0; e < coded; ++e) {
