@@ -1243,7 +1243,8 @@ Plan plan_of(const D8sCacheAttnArgs* a) {
     const bool tile = rows >= 64 && heads * ((rows + 15) / 16) * seen(16) > 12000;
     const int64_t each = !tile ? 16 : rows <= 128 || seen(128) < 32 ? 128 : 256, tiles = (rows + each - 1) / each, problems = heads * tiles, blocks = seen(each);
     const bool small = !tile && problems <= cus / 2 && blocks <= (a->c.D == 64 ? 3 * SMALL<64> : 2 * SMALL<128>);
-    if (!tile && !small && tiles == 1 && a->c.B > 1 && a->c.B <= EVEN_ROWS && blocks >= 16 && 4 * blocks > 3 * (a->c.S / BLK))
+    const bool joined = (int64_t)a->c.B * a->T * a->H < (1 << 24);           // (a workgroup a row: fewer than 2^32 threads)
+    if (!tile && !small && tiles == 1 && a->c.B > 1 && a->c.B <= EVEN_ROWS && joined && blocks >= 16 && 4 * blocks > 3 * (a->c.S / BLK))
         return {false, true, 16, 1, (int)std::max<int64_t>(1, std::min(2 * cus, problems * blocks / 4))};
     const int64_t slots = each == 256 ? (a->c.D == 64 ? 2 * cus : cus) : 2 * cus;
     const int64_t split = small ? 1 : tile ? std::min(slots / problems, blocks / 8) : std::min(slots / problems - 1, blocks / 4);
