@@ -316,28 +316,30 @@ __global__ __launch_bounds__(1024) void k_grad_norm(const double* part, int n, L
 // workgroup, which saves the launch between (22 tensors of 1.4 M elements: 31 -> 27 us with the host's work).
 // (From the last chunk to the first, for what the last-level cache still holds of the norm's reads, and with stores past that
 // cache: no change.)
-constexpr int FEW = 256;
+constexpr int FEW = 256, SCALE_WGS = 1 << 23;  // (a launch has fewer than 2^24 workgroups of 256 threads)
 template <class G>
 __global__ __launch_bounds__(256) void k_grad_scale(Grads t, const double* part, int n, Limit limit, bool keep) {
     constexpr int V = 16 / sizeof(G), TURNS = CHUNK / (256 * V);
     const float by = n <= FEW ? norm_factor<256>(part, n, limit, keep && blockIdx.x == 0) : *limit.factor;
     if (by == 1.0f) return;
-    const int c = blockIdx.x, i = tensor_of(t, c);
-    const int64_t at = (int64_t)(c - t.first[i]) * CHUNK;
-    G* g = (G*)t.g[i] + at;
-    const int64_t left = t.n[i] - at;
-    if (left >= CHUNK) {
-        Vec<G, V> x[TURNS];
+    for (int c = blockIdx.x, all = t.first[t.count]; c < all; c += gridDim.x) {
+        const int i = tensor_of(t, c);
+        const int64_t at = (int64_t)(c - t.first[i]) * CHUNK;
+        G* g = (G*)t.g[i] + at;
+        const int64_t left = t.n[i] - at;
+        if (left >= CHUNK) {
+            Vec<G, V> x[TURNS];
 #pragma unroll
-        for (int k = 0; k < TURNS; ++k) x[k] = *(const Vec<G, V>*)(g + (k * 256 + threadIdx.x) * V);
+            for (int k = 0; k < TURNS; ++k) x[k] = *(const Vec<G, V>*)(g + (k * 256 + threadIdx.x) * V);
 #pragma unroll
-        for (int k = 0; k < TURNS; ++k) {
+            for (int k = 0; k < TURNS; ++k) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) x[k][j] = (G)((float)x[k][j] * by);
-            *(Vec<G, V>*)(g + (k * 256 + threadIdx.x) * V) = x[k];
+                for (int j = 0; j < V; ++j) x[k][j] = (G)((float)x[k][j] * by);
+                *(Vec<G, V>*)(g + (k * 256 + threadIdx.x) * V) = x[k];
+            }
+        } else {
+            for (int k = threadIdx.x; k < left; k += 256) g[k] = (G)((float)g[k] * by);
         }
-    } else {
-        for (int k = threadIdx.x; k < left; k += 256) g[k] = (G)((float)g[k] * by);
     }
 }
 
@@ -516,7 +518,7 @@ extern "C" int d8s_grad_clip(const D8sGradNormArgs* a, void* stream) {
     if (parts > FEW || n == 0) hipLaunchKernelGGL(k_grad_norm, dim3(1), dim3(1024), 0, st, part, parts, limit);
     bool keep = true;                          // (the first of the launches leaves the norm)
     grad_launches(a->tensors, a->count, [&](const Grads& t, int dtype) {
-        const dim3 grid((unsigned)t.first[t.count]);
+        const dim3 grid((unsigned)std::min(t.first[t.count], SCALE_WGS));
         if (dtype == D8S_F32) hipLaunchKernelGGL(k_grad_scale<float>, grid, dim3(256), 0, st, t, part, parts, limit, keep);
         else if (dtype == D8S_BF16) hipLaunchKernelGGL(k_grad_scale<bf16>, grid, dim3(256), 0, st, t, part, parts, limit, keep);
         else hipLaunchKernelGGL(k_grad_scale<f16>, grid, dim3(256), 0, st, t, part, parts, limit, keep);
