@@ -223,12 +223,14 @@ DEV float value_of(uint32_t word, int k) {
     else return (float)((int)byte - 128);
 }
 
+constexpr int READ_WGS = 1 << 23;              // in a row of the grid (one dimension has fewer than 2^32 threads)
 template <class T, class O, bool E4M3, int D>
 __global__ __launch_bounds__(NT) void k_cache_read(D8sCacheReadArgs p, int blocks) {
     constexpr int P = D / 8, N = D / 32, PITCH = BLK + 4;
     __shared__ uint32_t turned[D * PITCH / 4];
     const D8sCache& c = p.c;
-    const int id = blockIdx.x, hk = id % c.HK, values = id / c.HK & 1, j = id / c.HK / 2 % blocks, b = id / c.HK / 2 / blocks;
+    const int id = blockIdx.y * READ_WGS + blockIdx.x, hk = id % c.HK, values = id / c.HK & 1, j = id / c.HK / 2 % blocks, b = id / c.HK / 2 / blocks;
+    if (b >= c.B) return;
     const int n = length_of(c, b), nb = c.S / BLK;
     const int64_t head = (int64_t)b * c.HK + hk, block = head * nb + j;
     const int ch = threadIdx.x % P * 8, t0 = threadIdx.x / P * N;
@@ -1275,7 +1277,8 @@ void append_run(const D8sCacheAppendArgs& a, hipStream_t st) {
 template <class T, bool E4M3, int D>
 void read_run(const D8sCacheReadArgs& a, hipStream_t st) {
     const int blocks = (a.tokens + BLK - 1) / BLK;
-    const dim3 grid((unsigned)((int64_t)a.c.B * a.c.HK * 2 * blocks));
+    const int64_t all = (int64_t)a.c.B * a.c.HK * 2 * blocks;
+    const dim3 grid((unsigned)std::min<int64_t>(all, READ_WGS), (unsigned)((all + READ_WGS - 1) / READ_WGS));
     if (a.out_dtype == D8S_F32) hipLaunchKernelGGL((k_cache_read<T, float, E4M3, D>), grid, dim3(NT), 0, st, a, blocks);
     else hipLaunchKernelGGL((k_cache_read<T, T, E4M3, D>), grid, dim3(NT), 0, st, a, blocks);
 }
@@ -1352,7 +1355,7 @@ extern "C" int d8s_cache_read(const D8sCacheReadArgs* a, void* stream) {
     if (int rc = cache_check(&a->c, what)) return rc;
     CREQ(a->tokens >= 1 && a->tokens <= a->c.S, "tokens must be 1 .. S");
     CREQ(a->out_dtype == D8S_F32 || a->out_dtype == a->c.dtype, "out_dtype must be D8S_F32 or dtype");
-    CREQ((int64_t)a->c.B * a->c.HK * 2 * ((a->tokens + BLK - 1) / BLK) < (1 << 24), "too many heads and tokens");
+    CREQ((int64_t)a->c.B * a->c.HK * 2 * ((a->tokens + BLK - 1) / BLK) < (1ll << 31) - READ_WGS, "too many heads and tokens");
     CREQ(a->k && a->v, "null pointer");
     BY_KIND(read_run, *a, (hipStream_t)stream);
     return d8s_host_launched(what);

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from rsna_knee_efficiency_amd import optim
+from rsna_knee_efficiency_amd.token_cache import QuantizedCache
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +39,16 @@ def test_clipping_of_a_tensor_of_half_the_limit(dev, free):
     assert optim.clip_grad_norm([x], 0.5).item() == torch.tensor(math.sqrt(len(at))).item()
     want = torch.tensor(0.5 / math.sqrt(len(at))).bfloat16().item()
     assert [x[i].item() for i in at] == [want] * len(at) and not x[-3:-1].any() and not x[1:8191].any()
+
+
+def test_reading_all_of_a_large_cache(dev, free):
+    """2^24 workgroups: a row that is full and one of 200 tokens"""
+    n = 1 << 28
+    free(n * 128 * 6)                          # (two rows of 64 channels: codes in 8 bits, and what is read in 16)
+    cache = QuantizedCache(2, n, 1, 64, device=dev)
+    x = torch.full((1, 1, 1, 64), 1.5, dtype=torch.bfloat16, device=dev).expand(2, n, 1, 64)
+    cache.append(x, -x[:, :1].expand(2, n, 1, 64), torch.tensor([200, n], dtype=torch.int32, device=dev))
+    print("read 2^28 tokens of two rows", flush=True)
+    for got, want in zip(cache.read(), (1.5, -1.5)):
+        assert (got[0, :200] == want).all() and not got[0, 200:1 << 20].any() and not got[0, 200::4097].any() and not got[0, -(1 << 20):].any()
+        assert (got[1, :1 << 20] == want).all() and (got[1, ::4097] == want).all() and (got[1, -(1 << 20):] == want).all()
