@@ -20,6 +20,8 @@ import torch
 from . import hip
 from .context import _extent, _fail, _last, _like, _no_tangents, _on_gpu
 
+_BLOCK = hip.CACHE_BLOCK
+
 
 def _no_gradients(*tensors: torch.Tensor) -> None:
     _no_tangents(*tensors)
@@ -56,6 +58,8 @@ class QuantizedCache:
             _fail("batch, capacity and key_heads must be positive")
         if capacity > 1 << 29:
             _fail("at most 2^29 tokens")
+        if batch * key_heads >= 1 << 22:
+            _fail("too many heads: batch times key_heads must be below 2^22")
         if channels not in (64, 128):
             _fail("64 or 128 channels a head")
         if codes not in hip.CODES:
@@ -67,7 +71,7 @@ class QuantizedCache:
             _fail("the cache must be on a GPU")
         self.batch, self.capacity, self.key_heads, self.channels, self.codes, self.dtype = (
             batch, capacity, key_heads, channels, codes, dtype)
-        block, blocks = hip.CACHE_BLOCK, max(1, capacity // hip.CACHE_BLOCK)
+        block, blocks = _BLOCK, max(1, capacity // _BLOCK)
 
         def empty(*shape, of):
             return torch.empty((batch, key_heads, *shape), dtype=of, device=device)
@@ -95,13 +99,15 @@ class QuantizedCache:
     def append(self, k: torch.Tensor, v: torch.Tensor, counts: torch.Tensor | None = None) -> None:
         """Appends k and v (batch, tokens, key heads, channels) in the cache's dtype, any strides (the channels are copied
         where they are not contiguous).  counts (batch,) int32 on the GPU: only the first counts[b] (taken as 0 .. tokens)
-        are there.  One launch; calls on one cache must follow each other."""
+        are there.  One launch; calls on one cache must follow each other.  (At most 2^29 tokens, and 2^24 blocks of all heads.)"""
         _no_gradients(k, v)
         shape = (self.batch, k.shape[1] if k.dim() == 4 else 0, self.key_heads, self.channels)
         if k.shape != shape or v.shape != shape:
             _fail(f"k and v must be ({self.batch}, tokens, {self.key_heads}, {self.channels})")
         if k.dtype != self.dtype or v.dtype != self.dtype:
             _fail("k and v must have the cache's dtype")
+        if shape[1] > 1 << 29 or self.batch * self.key_heads * ((shape[1] + 2 * _BLOCK - 2) // _BLOCK) >= 1 << 24:
+            _fail("too many heads and tokens for one call")
         _on_gpu(self._lengths, k, v)
         counts = _counts(counts, self.batch, self._lengths)
         if not shape[1]:
@@ -162,6 +168,8 @@ def cached_attention(q: torch.Tensor, cache: QuantizedCache, left: int | None = 
         _fail(f"q must be ({cache.batch}, tokens, heads, {cache.channels}), heads a multiple of {cache.key_heads}")
     if q.dtype != cache.dtype:
         _fail("q must have the cache's dtype")
+    if q.numel() // cache.channels >= 1 << 27:
+        _fail("too many heads and tokens for one call: batch times tokens times heads must be below 2^27")
     _on_gpu(cache._lengths, q)
     counts = _counts(counts, cache.batch, cache._lengths)
     scale = 1.0 / math.sqrt(cache.channels) if scale is None else float(scale)
