@@ -111,8 +111,9 @@ class ContextLayer:
         recorded into a graph: every replay appends behind the one before."""
         x = x.to(self.dtype)
         q, k, v = self._project(x, positions)
+        args = token_cache.checked(q, cache, self.left, self.right, self.sinks, counts)    # (a call that is refused appends nothing)
         cache.append(k, v, counts)
-        return self._rest(x, token_cache.cached_attention(q, cache, self.left, self.right, self.sinks, counts))
+        return self._rest(x, token_cache.attend(q, cache, *args))
 
     @torch.no_grad()
     def token(self, x: torch.Tensor, positions: torch.Tensor, cache: TokenCache | token_cache.QuantizedCache) -> torch.Tensor:

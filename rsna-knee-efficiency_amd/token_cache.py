@@ -152,17 +152,10 @@ def _workspace(device: torch.device, sizes: tuple, T: int, H: int, left: int, ri
     return need.value
 
 
-def cached_attention(q: torch.Tensor, cache: QuantizedCache, left: int | None = None, right: int | None = 0, sinks: int = 0,
-                     counts: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
-    """Attention of new tokens over a cache that holds them already: q (batch, tokens, heads, channels) in the cache's dtype are
-    the queries of every row's last tokens, or, with counts (batch,) int32 on the GPU (taken as 0 .. tokens), the first
-    counts[b] of them are.  Query head h uses key head h // (heads / key heads).
-
-    The token at position i of its row sees token j iff j <= i + right, and j >= i - left or j < sinks (None: no limit on that
-    side): as in `context.window_attention` over all of the row.  -> out like q: zeros for a query that sees nothing or is past
-    its row's count.  scale: 1 / sqrt(channels) unless given (2^-100 .. 2^100).  (A value of the last, 16-bit block that is not
-    finite can spoil the queries beside those that see it.  A query that sees bfloat16 values above 2^64, or some token of a full
-    block that has one, loses digits of what others below 2^-70 add to its result.)"""
+def checked(q: torch.Tensor, cache: QuantizedCache, left: int | None, right: int | None, sinks: int,
+            counts: torch.Tensor | None, scale: float | None = None) -> tuple:
+    """`cached_attention`'s checks of its arguments -> the others of `attend`.  (Apart, for a caller that appends between them: a call that
+    is refused should leave the cache as it was.)"""
     _no_gradients(q)
     if q.dim() != 4 or q.shape[0] != cache.batch or q.shape[3] != cache.channels or q.shape[2] < 1 or q.shape[2] % cache.key_heads:
         _fail(f"q must be ({cache.batch}, tokens, heads, {cache.channels}), heads a multiple of {cache.key_heads}")
@@ -175,7 +168,11 @@ def cached_attention(q: torch.Tensor, cache: QuantizedCache, left: int | None = 
     scale = 1.0 / math.sqrt(cache.channels) if scale is None else float(scale)
     if not 2.0 ** -100 <= scale <= 2.0 ** 100:
         _fail("scale must be positive: 2^-100 .. 2^100")
-    left, right, sinks = _extent(left, "left"), _extent(right, "right"), _extent(sinks, "sinks")
+    return _extent(left, "left"), _extent(right, "right"), _extent(sinks, "sinks"), counts, scale
+
+
+def attend(q: torch.Tensor, cache: QuantizedCache, left: int, right: int, sinks: int, counts: torch.Tensor | None, scale: float) -> torch.Tensor:
+    """`cached_attention` of arguments that `checked` has returned"""
     out = _like(q)
     if not q.numel():
         return out
@@ -188,3 +185,17 @@ def cached_attention(q: torch.Tensor, cache: QuantizedCache, left: int | None = 
         made, q.data_ptr(), 0 if counts is None else counts.data_ptr(), out.data_ptr(), 0 if work is None else work.data_ptr(),
         need, *q.stride()[:3], T, H, left, right, sinks, scale))
     return out
+
+
+def cached_attention(q: torch.Tensor, cache: QuantizedCache, left: int | None = None, right: int | None = 0, sinks: int = 0,
+                     counts: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+    """Attention of new tokens over a cache that holds them already: q (batch, tokens, heads, channels) in the cache's dtype are
+    the queries of every row's last tokens, or, with counts (batch,) int32 on the GPU (taken as 0 .. tokens), the first
+    counts[b] of them are.  Query head h uses key head h // (heads / key heads).
+
+    The token at position i of its row sees token j iff j <= i + right, and j >= i - left or j < sinks (None: no limit on that
+    side): as in `context.window_attention` over all of the row.  -> out like q: zeros for a query that sees nothing or is past
+    its row's count.  scale: 1 / sqrt(channels) unless given (2^-100 .. 2^100).  (A value of the last, 16-bit block that is not
+    finite can spoil the queries beside those that see it.  A query that sees bfloat16 values above 2^64, or some token of a full
+    block that has one, loses digits of what others below 2^-70 add to its result.)"""
+    return attend(q, cache, *checked(q, cache, left, right, sinks, counts, scale))
