@@ -157,11 +157,12 @@ def checked(q: torch.Tensor, cache: QuantizedCache, left: int | None, right: int
     """`cached_attention`'s checks of its arguments -> the others of `attend`.  (Apart, for a caller that appends between them: a call that
     is refused should leave the cache as it was.)"""
     _no_gradients(q)
-    if q.dim() != 4 or q.shape[0] != cache.batch or q.shape[3] != cache.channels or q.shape[2] < 1 or q.shape[2] % cache.key_heads:
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != cache.batch or shape[3] != cache.channels or shape[2] < 1 or shape[2] % cache.key_heads:
         _fail(f"q must be ({cache.batch}, tokens, heads, {cache.channels}), heads a multiple of {cache.key_heads}")
     if q.dtype != cache.dtype:
         _fail("q must have the cache's dtype")
-    if q.numel() // cache.channels >= 1 << 27:
+    if shape[0] * shape[1] * shape[2] >= 1 << 27:
         _fail("too many heads and tokens for one call: batch times tokens times heads must be below 2^27")
     _on_gpu(cache._lengths, q)
     counts = _counts(counts, cache.batch, cache._lengths)
@@ -177,7 +178,7 @@ def attend(q: torch.Tensor, cache: QuantizedCache, left: int, right: int, sinks:
     if not q.numel():
         return out
     q = _last(q)
-    T, H = q.shape[1:3]
+    _, T, H, _ = q.shape
     made = cache._args()
     need = _workspace(cache.device, cache._sizes, T, H, left, right, sinks)
     work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
