@@ -789,8 +789,9 @@ __global__ __launch_bounds__(NT) void k_cache_even_join(D8sCacheAttnArgs p, Even
 // call a load and some shuffles: 8192 queries over themselves 566 -> 570, 4096 of 64 channels 105 -> 106.)
 //
 // Bound by its instructions: per 32 x 64 scores a wave issues 32 products of 32 cycles (D = 128) beside 218 vector instructions (32 of
-// them its share of the codes' conversion, at 128 rows 64), and two waves a SIMD overlap them in part: 2 x 256 queries of 32 heads over 22528
-// tokens of 8 key heads 198 .. 206 us, 0.92 .. 0.95 PFLOP/s (a large library product 1.36), the matrix unit 0.45 busy at 2.0 GHz.
+// them its share of the codes' conversion, at 128 rows 64), and two waves a SIMD hardly overlap them: 2 x 256 queries of 32 heads over 22528
+// tokens of 8 key heads 198 .. 206 us, 0.92 .. 0.95 PFLOP/s (a large library product 1.36), the matrix unit 0.45 busy, the vector unit 0.50, LDS
+// 0.28, at 2.0 GHz.
 // Tried, no better: crews of four waves a barrier apart, one at its products while the other forms weights (219 us: a lone wave's
 // weights wait for themselves); reads of LDS six products ahead by scheduling groups (204); a barrier for two blocks (192 .. 200).
 constexpr float VSPAN = 16.0f, SPREAD = 0x1p60f;
@@ -1228,6 +1229,8 @@ __global__ __launch_bounds__(NT) void k_cache_join(Part part, T* out) {
 //   28, and 23) or there are few blocks.
 // - Else every tile's blocks in as many shares as fill the GPU once (33 x 8192 tokens of one key head: 18.6, twice 23, four times 25;
 //   a few workgroups more than fit cost a round).
+// Lengths far below the capacity are run as if they filled it: 81 tokens over 1458 10.6 in a cache of 1458 tokens, 12.1 in one of 22528; calls
+// that the memory or the products bound take the same time in both (33 requests of 2048 tokens 17.4).
 template <int D>
 constexpr int SMALL = D == 64 ? 16 : 8;        // (registers for two or four waves a SIMD)
 struct Plan {
@@ -1237,7 +1240,8 @@ struct Plan {
 };
 Plan plan_of(const D8sCacheAttnArgs* a) {
     const int64_t rows = (int64_t)a->T * (a->H / a->c.HK), heads = (int64_t)a->c.B * a->c.HK, cus = d8s_host_cu_count();
-    const auto seen = [&](int64_t each) {      // blocks that a tile of so many rows sees, at most
+    const auto seen = [&](int64_t each) {      // about how many blocks a tile of so many rows sees in a full cache (one or two more where
+                                               // its window and the first tokens do not begin and end with a block)
         const int64_t tokens = (each - 1) / (a->H / a->c.HK) + 1;
         const int64_t wide = std::min<int64_t>(a->c.S, (int64_t)a->left + a->right + std::min<int64_t>(a->T, tokens));
         return (std::min<int64_t>(a->c.S, wide + a->sinks) + BLK - 1) / BLK;

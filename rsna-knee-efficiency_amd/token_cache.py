@@ -5,7 +5,8 @@
     cache.append(k, v)                                   # the keys and values of an image's tokens, or of one token
     out = cached_attention(q, cache, left=512, sinks=12)  # their queries over all that the cache holds
 
-Half the bytes of a 16-bit cache, and half the time of a token's attention, which is bound by reading it.  Calls run on
+Half the bytes of a 16-bit cache, and half the time of the attention of many requests' tokens, which is bound by reading it (64 requests of 8192
+tokens, 32 heads on 8 of 128 channels: 190 us, over a 16-bit cache 387; a single request's is a matter of latency, 13 and 14).  Calls run on
 the current stream of the cache's device and may be recorded into HIP graphs: lengths are kept on the GPU, so a replay
 appends its tokens behind those of the one before.  There is no CPU path: without the library the calls raise.  None
 of this has gradients (`context.window_attention` has): tensors that require one are refused outside `torch.no_grad()`.
