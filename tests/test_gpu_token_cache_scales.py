@@ -129,3 +129,42 @@ def test_tokens_of_the_last_block_that_a_row_does_not_see(dev, codes, d, batch, 
             cache.append(k, v.to(BF16))
             _check(cache, q)
             _check(cache, q, 40, 3, 2)
+
+
+@pytest.mark.parametrize("codes,d", [(INT8, 128), (E4M3, 64)])
+@pytest.mark.parametrize("new,h,hk", [(2500, 16, 4), (700, 64, 2), (45, 4, 2)])
+def test_ragged_requests_over_blocks_far_apart(dev, codes, d, new, h, hk):
+    """Requests of every length with some of the new tokens, among blocks of 2^120 and 2^-20 and one that is not a number: queries that
+    see nothing of it have their own results, those that see its value's block have none, what lies past a count is zeros and not read."""
+    g, n, left = torch.Generator(device=dev).manual_seed(new), 3000, 300
+    lengths, counts = [3000, 2000, 64, 0, 1700], [new, new // 3, 64, 5, 0]
+    b = len(lengths)
+    q, k = (torch.randn((b, t, heads, d), generator=g, device=dev).to(BF16) for t, heads in ((new, h), (n, hk)))
+    block = torch.arange(n, device=dev) // 64
+    v = (torch.rand((b, n, hk, d), generator=g, device=dev).double() * 2 - 1) * torch.exp2(torch.where(block % 4 == 1, 120.0, -20.0).double())[None, :, None, None]
+    v = v.to(BF16)
+    v[:, 64 * 25 + 7, 0, 3] = float("nan")
+    cache = QuantizedCache(b, n, hk, d, codes, BF16, dev)
+    cache.append(k, v, torch.tensor(lengths, dtype=torch.int32, device=dev))
+    for r, c in enumerate(counts):
+        q[r, c:] = float("nan")
+    print(f"ragged {codes} {d} new={new}", flush=True)
+    got = cached_attention(q, cache, left, 0, counts=torch.tensor(counts, dtype=torch.int32, device=dev))
+    kk, vv = cache.read(dtype=F32)
+    for r, (m, c) in enumerate(zip(lengths, counts)):
+        c = min(c, new)
+        assert not got[r, c:].any()
+        s = min(c, m)
+        if not s:
+            assert not got[r].any()
+            continue
+        at = torch.arange(m - s, m, device=dev)
+        sees = (at >= 64 * 25) & (at - left < 64 * 26) & (m >= 64 * 26)
+        want, tol = _oracle(q[r, c - s:c], kk[r, :m], vv[r, :m].nan_to_num(0.0), left, 0, 0, d ** -0.5)
+        mine, per = got[r, c - s:c], h // hk
+        bad = torch.zeros((s, h), dtype=torch.bool, device=dev)
+        bad[:, :per] = sees[:, None]
+        assert mine[bad].isnan().all()
+        assert ((mine.double() - want).abs() <= tol)[~bad].all()
+        if c > s:
+            assert not got[r, :c - s].any()
